@@ -55,6 +55,12 @@ typedef enum {
   PK_I8 = 5
 } pk_dtype;
 
+/* Activations of the gated product. */
+typedef enum {
+  PK_ACT_SILU = 0,      /* g / (1 + exp(-g)) */
+  PK_ACT_GELU_TANH = 1  /* g / 2 * (1 + tanh(sqrt(2/pi) * (g + 0.044715 g^3))) */
+} pk_act;
+
 /* Library version (major*10000 + minor*100 + patch). */
 PK_API int pk_version(void);
 
@@ -360,6 +366,62 @@ PK_API size_t pk_gemm_splitk_workspace_size(int64_t M, int64_t N, int64_t K, int
  * reduces with fp32 atomics into a zeroed C (gemm_splitk.py:64,72). */
 PK_API int pk_gemm_splitk(const void* a, const void* b, int dtype, int64_t M, int64_t N, int64_t K,
                    int split_k, float* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* W8A8: rows in 8 bits with one scale each, and their products            */
+/* ---------------------------------------------------------------------- */
+/* No counterparts in the reference. 8-bit operands (dtype I8 or E4M3) are
+ * rows of K consecutive codes, `ld` codes apart, with x ~= code * scale[row]:
+ * activations one row per token, weights [N, K] one row per output channel
+ * (nn.Linear's own layout). Calls on one stream may be captured in CUDA
+ * graphs; none needs a workspace, so captured graphs share nothing. */
+
+/* Per-row symmetric quantization of x[M, K] (dtype F16/BF16/F32, ld ldx):
+ *   a = max(max_k |x[m, k]|, 1e-12),  scale[m] = a / most,
+ *   q[m, k] = round_half_even(x[m, k] * (most / a)),  most = 127 (I8), 448 (E4M3)
+ * in fp32. A row with a NaN or an infinity gets scale NaN and codes 0. K < 2^30. */
+PK_API int pk_quantize_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
+                            int q_dtype, int64_t ldq, float* scale, void* stream);
+
+/* out[m, k] = q[m, k] * scale[m], the product in fp32, rounded once to
+ * out_dtype (F16/BF16/F32). */
+PK_API int pk_dequantize_rows(const void* q, int q_dtype, int64_t M, int64_t K, int64_t ldq,
+                              const float* scale, void* out, int out_dtype, int64_t ldo,
+                              void* stream);
+
+/* Root-mean-square norm with the residual's addition and an 8-bit output:
+ *   h = x + residual in x's type (h = x when residual is NULL),
+ *   y = h / sqrt(mean_k(h^2) + eps) * weight,
+ * and y's rows quantized as pk_quantize_rows does (sums and y in fp32). x,
+ * residual, h: dtype F16/BF16/F32; weight[K]: that type or F32. h (required
+ * with a residual, ignored without) receives the sum and may be x or residual
+ * itself (same pointer and leading dimension), but overlaps them in no other
+ * way. eps is at least the smallest normal fp32 number. */
+PK_API int pk_rms_norm_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                             const void* residual, int64_t ldr, const void* weight, int w_dtype,
+                             float eps, void* h, int64_t ldh, void* q, int q_dtype, int64_t ldq,
+                             float* scale, void* stream);
+
+/* out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n] + bias[n]
+ * (bias: fp32 [N] or NULL). a and w both I8 (summed exactly in int32; K <=
+ * 131071) or both E4M3 (fp32 sums); the scales multiply in fp32 in the order
+ * written; out F32, BF16 or F16 (ld ldo). a and w are 16-byte aligned with lda
+ * and ldw multiples of 16 (K itself is free; what lies between K and ld is not
+ * read). */
+PK_API int pk_w8a8_gemm(const void* a, int ab_dtype, int64_t lda, const float* a_scale,
+                        const void* w, int64_t ldw, const float* w_scale, const float* bias,
+                        int64_t M, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                        void* stream);
+
+/* Both input projections of a gated feed-forward block, its activation and
+ * the product, in one kernel: out[m, n] = act(g) * u with g and u the products
+ * pk_w8a8_gemm defines for w_gate and w_up (both [N, K]); activation a pk_act.
+ * g, u and the activation are fp32; one rounding to out_dtype. */
+PK_API int pk_w8a8_gated_gemm(const void* a, int ab_dtype, int64_t lda, const float* a_scale,
+                              const void* w_gate, int64_t ld_gate, const float* gate_scale,
+                              const void* w_up, int64_t ld_up, const float* up_scale,
+                              int activation, int64_t M, int64_t N, int64_t K, void* out,
+                              int out_dtype, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

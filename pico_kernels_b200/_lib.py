@@ -79,6 +79,14 @@ SIGNATURES = {
                                      _int, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
     "pk_fake_quant_groups": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp]),
     "pk_gptq_ref": (_int, [_vp, _vp, _i64, _i64, _int, _int, _vp, _vp]),
+    "pk_quantize_rows": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp]),
+    "pk_dequantize_rows": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _i64, _vp]),
+    "pk_rms_norm_quant": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _int, _f32, _vp,
+                                 _i64, _vp, _int, _i64, _vp, _vp]),
+    "pk_w8a8_gemm": (_int, [_vp, _int, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp,
+                            _int, _i64, _vp]),
+    "pk_w8a8_gated_gemm": (_int, [_vp, _int, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _int,
+                                  _i64, _i64, _i64, _vp, _int, _i64, _vp]),
     "pk_set_wait_limit_ns": (_int, [_i64]),
     "pk_set_weight_staging": (_int, [_int]),
     "pk_debug_phase_stamps": (_int, [_vp, _sz]),
@@ -198,6 +206,18 @@ def require_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_cuda:
             raise DtypeError("pico_kernels_b200 runs on CUDA tensors only (no CPU path)")
+
+
+def require_same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise DtypeError(f"tensors on different devices ({first.device} and {t.device})")
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (kernels launch on
+    the current device, whatever stream they are given)."""
+    return torch.cuda.device(t.device)
 
 
 def device_status(reset: bool = True) -> tuple[int, int]:

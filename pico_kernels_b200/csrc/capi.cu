@@ -1,6 +1,7 @@
 // extern "C" entry points of libpico_b200.so (declared in include/pico_b200.h):
 // argument validation, path selection, tensor-map encoding, the device status
 // word and the per-thread error message.
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -696,6 +697,58 @@ int sharded_path(int64_t M, int64_t N, int64_t K, int group, bool grouped, int o
 
 }  // namespace
 
+namespace {
+
+// Sizes and code type of 8-bit rows.
+int check_rows8(int64_t M, int64_t K, int q_dtype) {
+  if (M <= 0 || K <= 0) return fail(PK_ERR_SHAPE, "need M, K > 0");
+  if (K >= (1ll << 30) || M >= (1ll << 31) - 1) return fail(PK_ERR_SHAPE, "dimension too large");
+  if (q_dtype != PK_I8 && q_dtype != PK_E4M3)
+    return fail(PK_ERR_DTYPE, "8-bit rows are int8 or e4m3");
+  return PK_OK;
+}
+
+// int32 holds K products of magnitude up to 2^14
+constexpr int64_t kMaxInt8K = (1ll << 17) - 1;
+
+int run_w8a8(W8A8Args& g, int dtype, cudaStream_t s) {
+  const int weights = g.gated ? 2 : 1;
+  if (!g.a || !g.a_scale || !g.out) return fail(PK_ERR_SHAPE, "null pointer");
+  for (int i = 0; i < weights; ++i)
+    if (!g.w[i] || !g.w_scale[i]) return fail(PK_ERR_SHAPE, "null pointer");
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0) return fail(PK_ERR_SHAPE, "need M, N, K > 0");
+  if (g.M >= (1ll << 30) || g.N >= (1ll << 30) || g.K >= (1ll << 30))
+    return fail(PK_ERR_SHAPE, "dimension too large");
+  if (dtype != PK_I8 && dtype != PK_E4M3)
+    return fail(PK_ERR_DTYPE, "W8A8 operands are both int8 or both e4m3");
+  if (g.out_dtype != PK_F32 && !is16(g.out_dtype))
+    return fail(PK_ERR_DTYPE, "output must be f32, bf16 or f16");
+  if (dtype == PK_I8 && g.K > kMaxInt8K)
+    return fail(PK_ERR_SHAPE, "int8 sums are exact for K <= %lld (got %lld)",
+                static_cast<long long>(kMaxInt8K), static_cast<long long>(g.K));
+  if (g.lda < g.K || g.ldo < g.N) return fail(PK_ERR_SHAPE, "leading dimension too small");
+  if ((reinterpret_cast<uintptr_t>(g.a) & 15) || g.lda % 16 != 0)
+    return fail(PK_ERR_ALIGN, "A must be 16-byte aligned with a leading dimension of 16 k");
+  for (int i = 0; i < weights; ++i) {
+    if (g.ldw[i] < g.K) return fail(PK_ERR_SHAPE, "leading dimension too small");
+    if ((reinterpret_cast<uintptr_t>(g.w[i]) & 15) || g.ldw[i] % 16 != 0)
+      return fail(PK_ERR_ALIGN, "weights must be 16-byte aligned with a leading dimension of 16 k");
+  }
+  const uintptr_t elt = g.out_dtype == PK_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(g.out) % elt != 0)
+    return fail(PK_ERR_ALIGN, "output must be aligned to its element");
+  g.e4m3 = dtype == PK_E4M3;
+  g.status = device_status_ptr();
+  const char* why = "";
+  cudaError_t e = launch_w8a8(g, s, &why);
+  if (e == cudaErrorInvalidValue && why[0] != '\0') return fail(PK_ERR_ALIGN, "%s", why);
+  if (e != cudaSuccess) return cuda_fail(e, "w8a8 gemm launch");
+  ok();
+  return PK_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int pk_fp8_gemm(const uint8_t* a8, const uint8_t* b8, int64_t M, int64_t N, int64_t K,
@@ -998,6 +1051,108 @@ int pk_gptq_ref(float* wt, const float* h_inv, int64_t K, int64_t N, int out_gro
   if (e != cudaSuccess) return cuda_fail(e, "gptq (reference rule) launch");
   ok();
   return PK_OK;
+}
+
+int pk_quantize_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
+                     int q_dtype, int64_t ldq, float* scale, void* stream) {
+  if (!x || !q || !scale) return fail(PK_ERR_SHAPE, "null pointer");
+  const int st = check_rows8(M, K, q_dtype);
+  if (st != PK_OK) return st;
+  if (ldx < K || ldq < K) return fail(PK_ERR_SHAPE, "leading dimension too small");
+  if (!is16(dtype) && dtype != PK_F32)
+    return fail(PK_ERR_DTYPE, "quantize_rows takes f16, bf16 or f32");
+  cudaError_t e = launch_quantize_rows(x, dtype, M, K, ldx, q, q_dtype == PK_E4M3, ldq, scale,
+                                       as_stream(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "quantize_rows launch");
+  ok();
+  return PK_OK;
+}
+
+int pk_dequantize_rows(const void* q, int q_dtype, int64_t M, int64_t K, int64_t ldq,
+                       const float* scale, void* out, int out_dtype, int64_t ldo, void* stream) {
+  if (!q || !scale || !out) return fail(PK_ERR_SHAPE, "null pointer");
+  const int st = check_rows8(M, K, q_dtype);
+  if (st != PK_OK) return st;
+  if (ldq < K || ldo < K) return fail(PK_ERR_SHAPE, "leading dimension too small");
+  if (!is16(out_dtype) && out_dtype != PK_F32)
+    return fail(PK_ERR_DTYPE, "dequantize_rows writes f16, bf16 or f32");
+  cudaError_t e = launch_dequantize_rows(q, q_dtype == PK_E4M3, M, K, ldq, scale, out, out_dtype,
+                                         ldo, as_stream(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dequantize_rows launch");
+  ok();
+  return PK_OK;
+}
+
+int pk_rms_norm_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                      const void* residual, int64_t ldr, const void* weight, int w_dtype, float eps,
+                      void* h, int64_t ldh, void* q, int q_dtype, int64_t ldq, float* scale,
+                      void* stream) {
+  if (!x || !weight || !q || !scale) return fail(PK_ERR_SHAPE, "null pointer");
+  if (residual && !h) return fail(PK_ERR_SHAPE, "a residual needs an output for the sum");
+  const int st = check_rows8(M, K, q_dtype);
+  if (st != PK_OK) return st;
+  if (ldx < K || ldq < K || (residual && (ldr < K || ldh < K)))
+    return fail(PK_ERR_SHAPE, "leading dimension too small");
+  if (!is16(dtype) && dtype != PK_F32)
+    return fail(PK_ERR_DTYPE, "rms_norm_quant takes f16, bf16 or f32");
+  if (w_dtype != dtype && w_dtype != PK_F32)
+    return fail(PK_ERR_DTYPE, "the norm weight must be f32 or of x's type");
+  if (!(eps >= FLT_MIN) || !(eps <= FLT_MAX))
+    return fail(PK_ERR_SHAPE, "eps must be a finite normal fp32 number > 0");
+  cudaError_t e = launch_rms_norm_quant(x, dtype, M, K, ldx, residual, ldr, weight,
+                                        w_dtype == PK_F32, eps, h, ldh, q, q_dtype == PK_E4M3, ldq,
+                                        scale, as_stream(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rms_norm_quant launch");
+  ok();
+  return PK_OK;
+}
+
+int pk_w8a8_gemm(const void* a, int ab_dtype, int64_t lda, const float* a_scale, const void* w,
+                 int64_t ldw, const float* w_scale, const float* bias, int64_t M, int64_t N,
+                 int64_t K, void* out, int out_dtype, int64_t ldo, void* stream) {
+  W8A8Args g{};
+  g.a = a;
+  g.lda = lda;
+  g.a_scale = a_scale;
+  g.w[0] = w;
+  g.ldw[0] = ldw;
+  g.w_scale[0] = w_scale;
+  g.bias = bias;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.out = out;
+  g.out_dtype = out_dtype;
+  g.ldo = ldo;
+  return run_w8a8(g, ab_dtype, as_stream(stream));
+}
+
+int pk_w8a8_gated_gemm(const void* a, int ab_dtype, int64_t lda, const float* a_scale,
+                       const void* w_gate, int64_t ld_gate, const float* gate_scale,
+                       const void* w_up, int64_t ld_up, const float* up_scale, int activation,
+                       int64_t M, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                       void* stream) {
+  if (activation != PK_ACT_SILU && activation != PK_ACT_GELU_TANH)
+    return fail(PK_ERR_SHAPE, "unknown activation %d", activation);
+  W8A8Args g{};
+  g.a = a;
+  g.lda = lda;
+  g.a_scale = a_scale;
+  g.w[0] = w_gate;
+  g.ldw[0] = ld_gate;
+  g.w_scale[0] = gate_scale;
+  g.w[1] = w_up;
+  g.ldw[1] = ld_up;
+  g.w_scale[1] = up_scale;
+  g.gated = true;
+  g.act = activation;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.out = out;
+  g.out_dtype = out_dtype;
+  g.ldo = ldo;
+  return run_w8a8(g, ab_dtype, as_stream(stream));
 }
 
 int pk_set_wait_limit_ns(int64_t ns) {

@@ -207,6 +207,37 @@ int64_t gemm_tiles(int64_t M, int64_t N);
 size_t gemm_splitk_workspace_bytes(int64_t M, int64_t N, int split);
 cudaError_t launch_gemm_tc(const GemmArgs& g, cudaStream_t s, const char** why);
 
+// ---- rows8.cu (8-bit rows: quantizer, its inverse, RMS norm with an 8-bit output)
+cudaError_t launch_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                 void* q, bool e4m3, int64_t ldq, float* scale, cudaStream_t s);
+cudaError_t launch_dequantize_rows(const void* q, bool e4m3, int64_t rows, int64_t cols,
+                                   int64_t ldq, const float* scale, void* out, int out_dtype,
+                                   int64_t ldo, cudaStream_t s);
+cudaError_t launch_rms_norm_quant(const void* x, int dtype, int64_t rows, int64_t cols,
+                                  int64_t ldx, const void* residual, int64_t ldr,
+                                  const void* weight, bool weight_f32, float eps, void* h,
+                                  int64_t ldh, void* q, bool e4m3, int64_t ldq, float* scale,
+                                  cudaStream_t s);
+
+// ---- w8a8_gemm.cu (8-bit products with a scale per token and channel) -----
+struct W8A8Args {
+  const void* a;             // [M, K] (ld lda), K contiguous
+  int64_t lda;
+  const float* a_scale;      // [M]
+  const void* w[2];          // [N, K]: the weights, or gate and up
+  int64_t ldw[2];
+  const float* w_scale[2];   // [N]
+  const float* bias;         // [N] or nullptr (not gated)
+  bool gated, e4m3;
+  int act;                   // pk_act (gated)
+  int64_t M, N, K;
+  void* out;
+  int out_dtype;             // PK_F32 / PK_BF16 / PK_F16
+  int64_t ldo;
+  int* status;
+};
+cudaError_t launch_w8a8(const W8A8Args& g, cudaStream_t s, const char** why);
+
 // ---- w4a16_simt.cu (any shape; CUDA cores) -------------------------------
 cudaError_t launch_w4a16_simt(const void* a, int a_dtype, int64_t lda, const uint8_t* wp,
                               const void* scales, float scalar_scale, int group, int64_t M,

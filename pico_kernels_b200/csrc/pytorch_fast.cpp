@@ -1,7 +1,7 @@
 // Torch-aware fast-call entry points (module pico_kernels_b200._pktorch).
 //
-// gemm_int4.int4_gemm and int4_gemm_host check a dozen tensor attributes
-// before their C-ABI call; on a slow host CPU each attribute read from Python
+// gemm_int4.int4_gemm and int4_gemm_host (and the W8A8 calls of gemm_w8a8 and
+// norm) check a dozen tensor attributes before their C-ABI call; on a slow host CPU each attribute read from Python
 // costs 0.1-0.3 us, together more than the decode GEMM's kernel. These
 // functions make the same checks on the tensors in C++ and call
 // libpico_b200.so directly (linked by its soname, so the library instance is
@@ -17,11 +17,13 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "pico_b200.h"
 
@@ -275,6 +277,296 @@ PyObject* int4_gemm_host(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// W8A8 (gemm_w8a8, norm). Served: CUDA tensors on the current device whose
+// strides the kernels read as they are. Outputs are allocated here.
+// ---------------------------------------------------------------------------
+int code8_of(at::ScalarType t) {
+  return t == at::kChar ? PK_I8 : t == at::kFloat8_e4m3fn ? PK_E4M3 : -1;
+}
+
+bool dtype_arg(PyObject* o, at::ScalarType* t) {
+  if (!THPDtype_Check(o)) return false;
+  *t = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  return true;
+}
+
+// A tensor on the current device, or nullptr.
+const at::Tensor* device_tensor(PyObject* o) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.is_cuda() && t.get_device() == c10::cuda::current_device() ? &t : nullptr;
+}
+
+at::TensorOptions on_device(const at::Tensor& like, at::ScalarType t) {
+  return at::TensorOptions().dtype(t).device(like.device());
+}
+
+void* stream_of(const at::Tensor& t) {
+  return reinterpret_cast<void*>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream());
+}
+
+int64_t pitch16(int64_t K) { return (K + 15) / 16 * 16; }
+
+// Contiguous rows of fp16 / bf16 / fp32 values, at least one row and column.
+bool value_rows(const at::Tensor& x, int64_t* rows, int64_t* K) {
+  if (code_of(x.scalar_type()) < 0 || x.dim() < 1 || !x.is_contiguous() || x.numel() == 0)
+    return false;
+  *K = x.size(-1);
+  *rows = x.numel() / *K;
+  return true;
+}
+
+// Storage of x's shape in 8-bit codes (rows 16 bytes' multiples apart) and one
+// scale per row.
+void empty_codes(const at::Tensor& x, int64_t K, at::ScalarType t, at::Tensor* q,
+                 at::Tensor* scale) {
+  const int64_t pitch = pitch16(K);
+  if (pitch == K) {
+    *q = at::empty(x.sizes(), on_device(x, t));
+  } else {
+    auto sizes = x.sizes().vec();
+    sizes.back() = pitch;
+    *q = at::empty(sizes, on_device(x, t)).narrow(-1, 0, K);
+  }
+  *scale = at::empty(x.sizes().slice(0, x.dim() - 1), on_device(x, at::kFloat));
+}
+
+PyObject* tuple_of(at::Tensor&& q, at::Tensor&& scale, PyObject* h) {
+  PyObject* a = THPVariable_Wrap(std::move(q));
+  PyObject* b = THPVariable_Wrap(std::move(scale));
+  PyObject* t = nullptr;
+  if (a != nullptr && b != nullptr)
+    t = h == nullptr ? PyTuple_Pack(2, a, b) : PyTuple_Pack(3, a, b, h);
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  Py_XDECREF(h);
+  return t;
+}
+
+// quantize_rows(x, dtype) -> (codes, scale), or the status, or -1
+PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) {
+    PyErr_Format(PyExc_TypeError, "quantize_rows takes 2 arguments (%zd given)", n);
+    return nullptr;
+  }
+  try {
+    const at::Tensor* x = device_tensor(args[0]);
+    at::ScalarType t;
+    int64_t rows, K;
+    if (x == nullptr || !dtype_arg(args[1], &t) || code8_of(t) < 0 || !value_rows(*x, &rows, &K))
+      return PyLong_FromLong(kNotServed);
+    at::Tensor q, scale;
+    empty_codes(*x, K, t, &q, &scale);
+    const int st = pk_quantize_rows(x->data_ptr(), code_of(x->scalar_type()), rows, K, K,
+                                    q.data_ptr(), code8_of(t), pitch16(K),
+                                    scale.data_ptr<float>(), stream_of(*x));
+    if (st != PK_OK) return PyLong_FromLong(st);
+    return tuple_of(std::move(q), std::move(scale), nullptr);
+  } catch (...) {
+    PyErr_Clear();
+    return PyLong_FromLong(kNotServed);
+  }
+}
+
+// One fp32 value per row, contiguous: `shape`, or `shape` with a trailing 1.
+const float* row_values(PyObject* o, int64_t rows) {
+  const at::Tensor* s = device_tensor(o);
+  if (s == nullptr || s->scalar_type() != at::kFloat || !s->is_contiguous() ||
+      s->numel() != rows || s->dim() < 1 || s->dim() > 2 || s->size(0) != rows)
+    return nullptr;
+  return s->data_ptr<float>();
+}
+
+// A 2-D 8-bit operand with rows the kernels can load, at least one of them.
+struct Codes {
+  const at::Tensor* t;
+  int64_t rows, K, pitch;
+  int code;
+};
+bool codes(PyObject* o, Codes* c) {
+  c->t = device_tensor(o);
+  if (c->t == nullptr) return false;
+  const at::Tensor& t = *c->t;
+  c->code = code8_of(t.scalar_type());
+  if (c->code < 0 || t.dim() != 2) return false;
+  c->rows = t.size(0);
+  c->K = t.size(1);
+  if (c->rows < 1 || c->K < 1) return false;
+  c->pitch = c->rows > 1 ? t.stride(0) : pitch16(c->K);
+  return (c->K == 1 || t.stride(1) == 1) && c->pitch % 16 == 0 && c->pitch >= c->K &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// dequantize_rows(codes, scale, dtype) -> values, or the status, or -1
+PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) {
+    PyErr_Format(PyExc_TypeError, "dequantize_rows takes 3 arguments (%zd given)", n);
+    return nullptr;
+  }
+  try {
+    Codes c;
+    at::ScalarType t;
+    if (!codes(args[0], &c) || !dtype_arg(args[2], &t) || code_of(t) < 0)
+      return PyLong_FromLong(kNotServed);
+    const float* scale = row_values(args[1], c.rows);
+    if (scale == nullptr) return PyLong_FromLong(kNotServed);
+    at::Tensor out = at::empty({c.rows, c.K}, on_device(*c.t, t));
+    const int st = pk_dequantize_rows(c.t->data_ptr(), c.code, c.rows, c.K, c.pitch, scale,
+                                      out.data_ptr(), code_of(t), c.K, stream_of(*c.t));
+    if (st != PK_OK) return PyLong_FromLong(st);
+    return THPVariable_Wrap(std::move(out));
+  } catch (...) {
+    PyErr_Clear();
+    return PyLong_FromLong(kNotServed);
+  }
+}
+
+// rms_norm_quant(x, weight, eps, residual, dtype, residual_out)
+//   -> (codes, scale[, h]), or the status, or -1
+PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_Format(PyExc_TypeError, "rms_norm_quant takes 6 arguments (%zd given)", n);
+    return nullptr;
+  }
+  try {
+    const at::Tensor* x = device_tensor(args[0]);
+    const at::Tensor* w = device_tensor(args[1]);
+    at::ScalarType t;
+    int64_t rows, K;
+    if (x == nullptr || w == nullptr || !PyFloat_Check(args[2]) || !dtype_arg(args[4], &t) ||
+        code8_of(t) < 0 || !value_rows(*x, &rows, &K))
+      return PyLong_FromLong(kNotServed);
+    if (w->dim() != 1 || w->size(0) != K || !w->is_contiguous() ||
+        (w->scalar_type() != x->scalar_type() && w->scalar_type() != at::kFloat))
+      return PyLong_FromLong(kNotServed);
+    const at::Tensor* r = nullptr;
+    if (args[3] != Py_None) {
+      r = device_tensor(args[3]);
+      if (r == nullptr || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes() ||
+          !r->is_contiguous())
+        return PyLong_FromLong(kNotServed);
+    }
+    at::Tensor h;
+    if (args[5] != Py_None) {
+      const at::Tensor* o = device_tensor(args[5]);
+      if (r == nullptr || o == nullptr || o->scalar_type() != x->scalar_type() ||
+          o->sizes() != x->sizes() || !o->is_contiguous())
+        return PyLong_FromLong(kNotServed);
+      // x, residual or a storage of its own: a partial overlap is refused in Python
+      for (const at::Tensor* in : {x, r, w})
+        if (o->is_alias_of(*in) && (in == w || o->data_ptr() != in->data_ptr()))
+          return PyLong_FromLong(kNotServed);
+      h = *o;
+    } else if (r != nullptr) {
+      h = at::empty(x->sizes(), on_device(*x, x->scalar_type()));
+    }
+    at::Tensor q, scale;
+    empty_codes(*x, K, t, &q, &scale);
+    const int st = pk_rms_norm_quant(
+        x->data_ptr(), code_of(x->scalar_type()), rows, K, K, r ? r->data_ptr() : nullptr, K,
+        w->data_ptr(), code_of(w->scalar_type()), static_cast<float>(PyFloat_AS_DOUBLE(args[2])),
+        r ? h.data_ptr() : nullptr, K, q.data_ptr(), code8_of(t), pitch16(K),
+        scale.data_ptr<float>(), stream_of(*x));
+    if (st != PK_OK) return PyLong_FromLong(st);
+    PyObject* ho = nullptr;
+    if (args[5] != Py_None) {
+      Py_INCREF(args[5]);
+      ho = args[5];
+    } else if (r != nullptr) {
+      ho = THPVariable_Wrap(std::move(h));
+      if (ho == nullptr) return nullptr;
+    }
+    return tuple_of(std::move(q), std::move(scale), ho);
+  } catch (...) {
+    PyErr_Clear();
+    return PyLong_FromLong(kNotServed);
+  }
+}
+
+// The output of a product: allocated, or `out_obj` (contiguous [M, N]).
+bool product_out(PyObject* dtype_obj, PyObject* out_obj, int64_t M, int64_t N,
+                 const at::Tensor& like, at::Tensor* y) {
+  at::ScalarType t;
+  if (!dtype_arg(dtype_obj, &t) || code_of(t) < 0) return false;
+  if (out_obj == Py_None) {
+    *y = at::empty({M, N}, on_device(like, t));
+    return true;
+  }
+  const at::Tensor* o = device_tensor(out_obj);
+  if (o == nullptr || o->scalar_type() != t || o->dim() != 2 || o->size(0) != M ||
+      o->size(1) != N || !o->is_contiguous())
+    return false;
+  *y = *o;
+  return true;
+}
+
+PyObject* product_result(int st, PyObject* out_obj, at::Tensor&& y) {
+  if (st != PK_OK) return PyLong_FromLong(st);
+  if (out_obj == Py_None) return THPVariable_Wrap(std::move(y));
+  Py_INCREF(out_obj);
+  return out_obj;
+}
+
+// w8a8_gemm(a8, a_scale, w8, w_scale, bias, out_dtype, out) -> y, or the status, or -1
+PyObject* w8a8_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) {
+    PyErr_Format(PyExc_TypeError, "w8a8_gemm takes 7 arguments (%zd given)", n);
+    return nullptr;
+  }
+  try {
+    Codes a, w;
+    if (!codes(args[0], &a) || !codes(args[2], &w) || a.code != w.code || a.K != w.K)
+      return PyLong_FromLong(kNotServed);
+    const float* sa = row_values(args[1], a.rows);
+    const float* sw = row_values(args[3], w.rows);
+    const float* bias = args[4] == Py_None ? nullptr : row_values(args[4], w.rows);
+    at::Tensor y;
+    if (sa == nullptr || sw == nullptr || (args[4] != Py_None && bias == nullptr) ||
+        !product_out(args[5], args[6], a.rows, w.rows, *a.t, &y))
+      return PyLong_FromLong(kNotServed);
+    const int st = pk_w8a8_gemm(a.t->data_ptr(), a.code, a.pitch, sa, w.t->data_ptr(), w.pitch, sw,
+                                bias, a.rows, w.rows, a.K, y.data_ptr(), code_of(y.scalar_type()),
+                                w.rows, stream_of(*a.t));
+    return product_result(st, args[6], std::move(y));
+  } catch (...) {
+    PyErr_Clear();
+    return PyLong_FromLong(kNotServed);
+  }
+}
+
+// w8a8_gated_gemm(a8, a_scale, w_gate, gate_scale, w_up, up_scale, activation,
+//                 out_dtype, out) -> y, or the status, or -1
+PyObject* w8a8_gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) {
+    PyErr_Format(PyExc_TypeError, "w8a8_gated_gemm takes 9 arguments (%zd given)", n);
+    return nullptr;
+  }
+  try {
+    Codes a, g, u;
+    if (!codes(args[0], &a) || !codes(args[2], &g) || !codes(args[4], &u) || a.code != g.code ||
+        a.code != u.code || a.K != g.K || a.K != u.K || g.rows != u.rows)
+      return PyLong_FromLong(kNotServed);
+    const float* sa = row_values(args[1], a.rows);
+    const float* sg = row_values(args[3], g.rows);
+    const float* su = row_values(args[5], u.rows);
+    const long act = PyLong_Check(args[6]) ? PyLong_AsLong(args[6]) : -1;
+    at::Tensor y;
+    if (sa == nullptr || sg == nullptr || su == nullptr ||
+        (act != PK_ACT_SILU && act != PK_ACT_GELU_TANH) ||
+        !product_out(args[7], args[8], a.rows, g.rows, *a.t, &y))
+      return PyLong_FromLong(kNotServed);
+    const int st = pk_w8a8_gated_gemm(a.t->data_ptr(), a.code, a.pitch, sa, g.t->data_ptr(),
+                                      g.pitch, sg, u.t->data_ptr(), u.pitch, su,
+                                      static_cast<int>(act), a.rows, g.rows, a.K, y.data_ptr(),
+                                      code_of(y.scalar_type()), g.rows, stream_of(*a.t));
+    return product_result(st, args[8], std::move(y));
+  } catch (...) {
+    PyErr_Clear();
+    return PyLong_FromLong(kNotServed);
+  }
+}
+
 // bind(workspaces): the dict of cached workspaces the Python path fills.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 1 || !PyDict_Check(args[0])) {
@@ -296,6 +588,26 @@ PyMethodDef kMethods[] = {
      reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(int4_gemm_host)), METH_FASTCALL,
      "int4_gemm_host(a, w_packed, scale, group_size, out, out_dtype): out, the C ABI's status "
      "on failure, or -1 when the Python path must take the call."},
+    {"quantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_rows)),
+     METH_FASTCALL,
+     "quantize_rows(x, dtype): (codes, scale), the C ABI's "
+     "status on failure, or -1 when the Python path must take the call."},
+    {"dequantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_rows)),
+     METH_FASTCALL,
+     "dequantize_rows(codes, scale, dtype): the values, the C ABI's "
+     "status on failure, or -1 when the Python path must take the call."},
+    {"rms_norm_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_quant)),
+     METH_FASTCALL,
+     "rms_norm_quant(x, weight, eps, residual, dtype, residual_out): (codes, scale[, h]), the C ABI's "
+     "status on failure, or -1 when the Python path must take the call."},
+    {"w8a8_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(w8a8_gemm)),
+     METH_FASTCALL,
+     "w8a8_gemm(a8, a_scale, w8, w_scale, bias, out_dtype, out): the output, the C ABI's "
+     "status on failure, or -1 when the Python path must take the call."},
+    {"w8a8_gated_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(w8a8_gated_gemm)),
+     METH_FASTCALL,
+     "w8a8_gated_gemm(a8, a_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype, out): the output, the C ABI's "
+     "status on failure, or -1 when the Python path must take the call."},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL,
      "bind(workspaces): the workspace dict of pico_kernels_b200._lib."},
     {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,337 @@
+"""The W8A8 products on the GPU against their definitions in 64 bits.
+
+Tolerances: int8 sums are exact, so a result carries the int32 -> fp32
+conversion, one product per scale and the bias's addition: four fp32 roundings
+(2^-24 each) of a magnitude of at most |sum| + |bias|, then the output type's
+half step. e4m3 sums are fp32: every addition may lose up to a last place
+(2^-23) of the running sum of magnitudes, K * 2^-23 * sum|a||w| at most, and
+the whole product stays within the framework's fp8 bar (rel-Frobenius 1e-5).
+The gated form carries both products' errors through act'(g) (at most 1.2 for
+SiLU and GELU) and u, and its own roundings: the exponent's relative error is
+|t| * 2^-22 where t < 0, a dozen roundings elsewhere.
+"""
+
+import pytest
+import torch
+
+import pico_kernels_b200 as pk
+from pico_kernels_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+CODES = [torch.int8, torch.float8_e4m3fn]
+# single tokens, a tile's edges in every dimension, lengths of one, odd sizes,
+# several waves of large tiles with a ragged last one
+SHAPES = [(1, 1, 1), (1, 4096, 4096), (1, 129, 1000), (2, 64, 15), (3, 1000, 17), (7, 128, 128),
+          (16, 256, 4096), (16, 8192, 1024), (17, 130, 127), (33, 1111, 1001), (64, 512, 129),
+          (65, 384, 640), (128, 2048, 256), (129, 257, 511), (200, 1000, 2048), (256, 256, 384),
+          (257, 31, 272), (300, 4096, 1024), (1000, 1111, 333), (1025, 8200, 192),
+          (5000, 520, 144), (40, 3, 20000)]
+
+
+def _codes(rows, cols, code, g, pitch=None):
+    v = torch.randn(rows, pitch or (cols + 15) // 16 * 16, device="cuda", generator=g)
+    most = 127 if code == torch.int8 else 448
+    v = (v * most / 4).clamp(-most, most)
+    return (v.round() if code == torch.int8 else v).to(code)[:, :cols]
+
+
+def _operands(M, N, K, code, seed=0, weights=1):
+    g = torch.Generator(device="cuda").manual_seed(seed + M + N + K)
+    most = 127 if code == torch.int8 else 448
+    a = _codes(M, K, code, g)
+    sa = (0.5 + torch.rand(M, device="cuda", generator=g)) * 4 / most
+    w = []
+    for _ in range(weights):
+        w += [_codes(N, K, code, g),
+              (0.5 + torch.rand(N, device="cuda", generator=g)) * 4 / most / K ** 0.5]
+    return a, sa, w, torch.randn(N, device="cuda", generator=g)
+
+
+def _product64(a, sa, w, sw):
+    """(product, its error bound before the bias and the output's rounding)."""
+    s = sa.double()[:, None] * sw.double()
+    y = (a.double() @ w.double().t()) * s
+    if a.dtype == torch.int8:
+        return y, 3 * U * y.abs()
+    mag = (a.double().abs() @ w.double().abs().t()) * s
+    return y, a.shape[1] * 2 * U * mag + 3 * U * y.abs()
+
+
+def _assert_near(y, ref, err, rel=None):
+    assert torch.isfinite(y.float()).all()
+    tol = err + HALF[y.dtype] * (ref.abs() + err) + TINY[y.dtype]
+    over = (y.double() - ref).abs() > tol
+    assert not over.any(), (over.sum().item(), (y.double() - ref).abs().max().item())
+    if rel is not None and y.dtype == torch.float32:
+        assert (torch.linalg.norm(y.double() - ref) <= rel * torch.linalg.norm(ref)).item()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_w8a8_gemm(M, N, K, code):
+    a, sa, (w, sw), b = _operands(M, N, K, code)
+    ref, err = _product64(a, sa, w, sw)
+    y = pk.w8a8_gemm(a, sa, w, sw)
+    assert y.dtype == torch.float32 and y.shape == (M, N)
+    _assert_near(y, ref, err, 1e-5)
+    assert torch.equal(pk.w8a8_gemm(a, sa, w, sw), y)
+    for dt in (torch.bfloat16, torch.float16):
+        # the fp32 result rounded once
+        assert torch.equal(pk.w8a8_gemm(a, sa, w, sw, out_dtype=dt), y.to(dt))
+    yb = pk.w8a8_gemm(a, sa, w, sw, bias=b)
+    _assert_near(yb, ref + b.double(), err + U * (ref.abs() + b.double().abs()))
+    assert pk.device_status() == (0, 0)
+
+
+def _act64(g, act):
+    if act == "silu":
+        return g * torch.sigmoid(g), g
+    t = 2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3)
+    return g * torch.sigmoid(t), t
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_w8a8_gated_gemm(M, N, K, code, act):
+    a, sa, (wg, sg, wu, su), _ = _operands(M, N, K, code, seed=1, weights=2)
+    (g, eg), (u, eu) = _product64(a, sa, wg, sg), _product64(a, sa, wu, su)
+    f, t = _act64(g, act)
+    ref = f * u
+    own = (12 + 4 * (-t).clamp(0, 100)) * U
+    err = 1.2 * eg * (u.abs() + eu) + f.abs() * eu + own * ref.abs()
+    y = pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su, activation=act)
+    _assert_near(y, ref, err, 1e-5)
+    for dt in (torch.bfloat16, torch.float16):
+        assert torch.equal(pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su, activation=act,
+                                              out_dtype=dt), y.to(dt))
+    assert pk.device_status() == (0, 0)
+
+
+def test_int8_sums_are_exact_to_the_last_unit():
+    # the largest K and the largest magnitudes: 131071 * 2^14 < 2^31
+    K = 131071
+    a = torch.full((2, K + 1), -128, device="cuda", dtype=torch.int8)[:, :K]
+    w = torch.full((3, K + 1), -128, device="cuda", dtype=torch.int8)[:, :K]
+    one = torch.ones(3, device="cuda")
+    for M in (2, 300):
+        x = a[:1].expand(M, K).contiguous()
+        x = torch.nn.functional.pad(x, (0, 1))[:, :K]
+        y = pk.w8a8_gemm(x, torch.ones(M, device="cuda"), w, one)
+        assert (y == float(K * 2 ** 14)).all()  # (2^17 - 1) * 2^14 is exact in fp32
+        x = x.clone()
+        x = torch.nn.functional.pad(x, (0, 1))[:, :K]
+        x[:, ::2] = 127
+        s = int((x[0].long() * w[0].long()).sum())
+        y = pk.w8a8_gemm(x, torch.ones(M, device="cuda"), w, one)
+        assert (y == torch.tensor(s, dtype=torch.float64).float().item()).all()
+
+
+def test_gate_far_from_zero():
+    # |g| from tiny to where exp leaves fp32: no NaN, act's own limits
+    vals = torch.tensor([0.0, 1e-30, -1e-30, 0.1, -0.1, 20.0, -20.0, 88.0, -88.0, -89.5, -104.0,
+                         3e4, -3e4, 1e12, -1e12, 1e30, -1e30], device="cuda")
+    n = vals.numel()
+    a = torch.ones(1, 16, device="cuda", dtype=torch.int8)
+    w = torch.zeros(n, 16, device="cuda", dtype=torch.int8)
+    w[:, 0] = 1
+    one = torch.ones(1, device="cuda")
+    for act in ("silu", "gelu_tanh"):
+        y = pk.w8a8_gated_gemm(a, one, w, vals, w, torch.ones(n, device="cuda"),
+                               activation=act)[0].double()
+        f, t = _act64(vals.double(), act)
+        assert torch.isfinite(y).all()
+        # below exp's range the result is zero or a subnormal: 1e-30 covers g * exp(-|t|) there
+        assert ((y - f).abs() <= (12 + 4 * (-t).clamp(0, 100)) * U * f.abs() + 1e-30).all()
+
+
+def test_scales_with_nan_reach_only_their_rows_and_columns():
+    a, sa, (w, sw), _ = _operands(200, 300, 256, torch.int8)
+    sa, sw = sa.clone(), sw.clone()
+    sa[7] = float("nan")
+    sw[11] = float("nan")
+    y = pk.w8a8_gemm(a, sa, w, sw)
+    bad = torch.isnan(y)
+    assert bad[7].all() and bad[:, 11].all()
+    assert bad.sum() == 200 + 300 - 1
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_layouts(code):
+    M, N, K = 70, 96, 208
+    g = torch.Generator(device="cuda").manual_seed(0)
+    wide = _codes(M, 512, code, g)
+    both = _codes(2 * N, K, code, g)
+    s = torch.rand(2 * N, device="cuda") / 100
+    sa = torch.rand(M, device="cuda") / 100
+    a = wide[:, 16:16 + K]                       # rows 512 apart, aligned
+    ref = pk.w8a8_gemm(a.contiguous(), sa, both[:N].clone(), s[:N].clone())
+    assert torch.equal(pk.w8a8_gemm(a, sa[:, None], both[:N], s[:N]), ref)
+    ug = wide[:, 7:7 + K]                        # unaligned: copied
+    assert torch.equal(pk.w8a8_gemm(ug, sa, both[:N], s[:N]),
+                       pk.w8a8_gemm(ug.contiguous(), sa, both[:N], s[:N]))
+    t = a.t().contiguous().t()                   # column-major
+    assert torch.equal(pk.w8a8_gemm(t, sa, both[:N], s[:N]), ref)
+    assert torch.equal(pk.w8a8_gemm(a[:1].expand(M, K), sa, both[:N], s[:N]),
+                       pk.w8a8_gemm(a[:1].repeat(M, 1), sa, both[:N], s[:N]))
+    # gate and up as halves of one weight
+    fused = pk.w8a8_gated_gemm(a, sa, both[:N], s[:N], both[N:], s[N:])
+    apart = pk.w8a8_gated_gemm(a, sa, both[:N].clone(), s[:N].clone(), both[N:].clone(),
+                               s[N:].clone())
+    assert torch.equal(fused, apart)
+    out = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+    assert pk.w8a8_gemm(a, sa, both[:N], s[:N], out_dtype=torch.bfloat16, out=out) is out
+    assert torch.equal(out, ref.bfloat16())
+    # no tokens
+    assert pk.w8a8_gemm(a[:0], sa[:0], both[:N], s[:N]).shape == (0, N)
+    assert pk.w8a8_gated_gemm(a[:0], sa[:0], both[:N], s[:N], both[N:], s[N:]).shape == (0, N)
+
+
+@pytest.mark.parametrize("M", [1, 5, 100, 700])
+def test_rows_and_columns_past_the_output_are_left_alone(M):
+    lib = _lib.load()
+    N, K, ldo = 200, 160, 264
+    a, sa, (w, sw), _ = _operands(M, N, K, torch.int8)
+    for dt, code in ((torch.float32, _lib.PK_F32), (torch.bfloat16, _lib.PK_BF16)):
+        buf = torch.full((M + 2, ldo), 77.0, device="cuda", dtype=dt)
+        st = lib.pk_w8a8_gemm(a.data_ptr(), _lib.PK_I8, a.stride(0), sa.data_ptr(), w.data_ptr(),
+                              w.stride(0), sw.data_ptr(), None, M, N, K, buf[1:].data_ptr(), code,
+                              ldo, _lib.stream_of(a))
+        assert st == _lib.PK_OK, _lib.last_error()
+        assert (buf[0] == 77).all() and (buf[-1] == 77).all() and (buf[:, N:] == 77).all()
+        assert torch.equal(buf[1:-1, :N], pk.w8a8_gemm(a, sa, w, sw, out_dtype=dt))
+        # an output whose rows are not 16-byte aligned
+        odd = torch.full((M * 203 + 1,), 77.0, device="cuda", dtype=dt)
+        st = lib.pk_w8a8_gemm(a.data_ptr(), _lib.PK_I8, a.stride(0), sa.data_ptr(), w.data_ptr(),
+                              w.stride(0), sw.data_ptr(), None, M, N, K, odd[1:].data_ptr(), code,
+                              203, _lib.stream_of(a))
+        assert st == _lib.PK_OK, _lib.last_error()
+        o = odd[1:].view(M, 203)
+        assert odd[0] == 77 and (o[:, N:] == 77).all()
+        assert torch.equal(o[:, :N], buf[1:-1, :N])
+
+
+def test_what_lies_between_the_columns_and_the_pitch_is_not_read():
+    for M in (3, 400):
+        a, sa, (w, sw), _ = _operands(M, 300, 100, torch.float8_e4m3fn)
+        ref = pk.w8a8_gemm(a, sa, w, sw)
+        for t in (a, w):
+            full = torch.as_strided(t.view(torch.uint8), (t.shape[0], t.stride(0)),
+                                    (t.stride(0), 1))
+            full[:, 100:] = 0x7F  # e4m3 NaN
+        assert torch.equal(pk.w8a8_gemm(a, sa, w, sw), ref)
+
+
+def test_output_offsets_past_31_bits():
+    M, N, K = 66000, 32768, 32
+    g = torch.Generator(device="cuda").manual_seed(0)
+    a, w = _codes(M, K, torch.int8, g), _codes(N, K, torch.int8, g)
+    sa, sw = torch.rand(M, device="cuda"), torch.rand(N, device="cuda")
+    y = pk.w8a8_gemm(a, sa, w, sw, out_dtype=torch.bfloat16)
+    tail = pk.w8a8_gemm(a[-200:], sa[-200:], w, sw, out_dtype=torch.bfloat16)
+    assert torch.equal(y[-200:], tail)
+
+
+def test_a_token_does_not_depend_on_its_batch_in_int8():
+    a, sa, (wg, sg, wu, su), b = _operands(600, 640, 512, torch.int8, weights=2)
+    y = pk.w8a8_gemm(a, sa, wg, sg, bias=b)
+    z = pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su)
+    for rows in (slice(0, 1), slice(5, 9), slice(100, 140), slice(300, 600)):
+        assert torch.equal(pk.w8a8_gemm(a[rows], sa[rows], wg, sg, bias=b), y[rows])
+        assert torch.equal(pk.w8a8_gated_gemm(a[rows], sa[rows], wg, sg, wu, su), z[rows])
+
+
+@pytest.mark.parametrize("M", [1, 12, 600])
+def test_fast_path_equals_python_path(M):
+    a, sa, (wg, sg, wu, su), b = _operands(M, 640, 520, torch.int8, weights=2)
+    tf = _lib.torch_fast()
+    assert tf is not None
+    y = tf.w8a8_gemm(a, sa, wg, sg, b, torch.bfloat16, None)
+    z = tf.w8a8_gated_gemm(a, sa, wg, sg, wu, su, 1, torch.float16, None)
+    assert isinstance(y, torch.Tensor) and isinstance(z, torch.Tensor)
+    saved = _lib._tfast
+    _lib._tfast = False
+    try:
+        assert torch.equal(pk.w8a8_gemm(a, sa, wg, sg, bias=b, out_dtype=torch.bfloat16), y)
+        assert torch.equal(pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su, activation="gelu_tanh",
+                                              out_dtype=torch.float16), z)
+    finally:
+        _lib._tfast = saved
+
+
+def _block(x, r, w, gate, up, down):
+    q, s, h = pk.rms_norm_quant(x, w, residual=r)
+    y = pk.w8a8_gated_gemm(q, s, *gate, *up, out_dtype=torch.bfloat16)
+    y8, sy = pk.quantize_rows(y)
+    return pk.w8a8_gemm(y8, sy, *down, out_dtype=torch.bfloat16), h
+
+
+def _block_weights(K, F, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (1 + 0.1 * torch.randn(K, device="cuda", generator=g)).bfloat16()
+    mats = [torch.randn(n, k, device="cuda", generator=g) * k ** -0.5
+            for n, k in ((F, K), (F, K), (K, F))]
+    return w, mats, [pk.quantize_rows(m) for m in mats]
+
+
+@pytest.mark.parametrize("M", [1, 16, 150, 600])
+def test_the_operators_together_as_a_feed_forward_block(M):
+    K, F = 1000, 1304
+    w, mats, packed = _block_weights(K, F)
+    x = torch.randn(M, K, device="cuda").bfloat16()
+    r = torch.randn(M, K, device="cuda").bfloat16()
+    y, h = _block(x, r, w, *packed)
+    assert torch.equal(h, (x.float() + r.float()).bfloat16())
+    # the float block: 8-bit codes are off by at most half a step of a row's
+    # 127th; with Gaussian rows (maximum ~3.5 deviations) that is ~0.8 % rms of
+    # each of the two operands of each product
+    n = h.double() / torch.sqrt(h.double().square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    g, u, d = (m.double() for m in mats)
+    t = torch.nn.functional.silu(n @ g.t()) * (n @ u.t())
+    ref = t @ d.t()
+    assert torch.linalg.norm(y.double() - ref) <= 0.05 * torch.linalg.norm(ref)
+    # the same chain of the operators' own values in 64 bits: what is left is
+    # bf16's rounding of y and the codes that a rounding moved by one
+    q, s = pk.rms_norm_quant(h, w)
+    n = q.double() * s.double()[:, None]
+    (g, u, d) = (pk.dequantize_rows(*p).double() for p in packed)
+    t8, st = pk.quantize_rows((torch.nn.functional.silu(n @ g.t()) * (n @ u.t())).bfloat16())
+    ref = (t8.double() * st.double()[:, None]) @ d.t()
+    assert torch.linalg.norm(y.double() - ref) <= 2.0 ** -8 * 2 * torch.linalg.norm(ref)
+    assert pk.device_status() == (0, 0)
+
+
+def test_block_captured_twice_and_replayed_at_once():
+    # nothing is shared between captured calls: two graphs of the same block run
+    # on two streams at the same time and give the eager results
+    w, _, packed = _block_weights(512, 768)
+    xs = [torch.randn(m, 512, device="cuda").bfloat16() for m in (1, 70)]
+    want = [_block(x, x, w, *packed) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_block(x, x, w, *packed))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, want_o in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, want_o))
+    for x in xs:
+        x.mul_(-1.5)
+    want = [_block(x, x, w, *packed) for x in xs]
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for o, want_o in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, want_o))
