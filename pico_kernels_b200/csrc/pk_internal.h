@@ -36,6 +36,12 @@ enum WaitSite : int {
   kSiteSkinnyMma = 402,
   kSiteSkinnyFinal = 403,
   kSiteSkinnyPeers = 404,
+  kSiteW8SwapProducer = 501,
+  kSiteW8SwapMma = 502,
+  kSiteW8SwapEpilogue = 503,
+  kSiteW8PairProducer = 511,
+  kSiteW8PairMma = 512,
+  kSiteW8PairEpilogue = 513,
 };
 
 // Host-side tensor map encoding (cuTensorMapEncodeTiled via the runtime's

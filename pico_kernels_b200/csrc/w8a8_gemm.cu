@@ -1,137 +1,713 @@
-// W8A8 products: out = (A8[M, K] @ W8[N, K]^T) * a_scale[m] * w_scale[n] (+ bias[n]),
-// and their gated form act(gate) * up of two such products.
+// W8A8 products for sm_100a: out[m, n] = (sum_k A8[m, k] W8[n, k]) * a_scale[m]
+// * w_scale[n] (+ bias[n]), and their gated form act(gate) * up.
 //
-// Simple form: one 64 x 64 output tile per CTA, 4 x 4 outputs per thread, the
-// operands staged 64 bytes of K at a time; int8 by four-way integer dot
-// products into int32 (exact), e4m3 by fp32 multiply-adds.
-#include <cuda_fp8.h>
+// int8 runs tcgen05 kind::i8 (int32 accumulators: exact), e4m3 runs
+// kind::f8f6f4 (fp32). Both operands are K-major rows, which is how TMA stages
+// them (128-byte swizzled tiles of 128 bytes of K) and the tensor core reads
+// them: no transposition, no conversion, no pass through registers. The
+// epilogue applies the scales in fp32 and rounds once to the output's type.
+//
+// Two kernels:
+//  * w8a8_swap_kernel, few tokens: the weights are the MMA's 128-row operand,
+//    the tokens its 16..256 columns, one tile per CTA. The product is a weight
+//    stream there; K is split over a thread-block cluster when there are too
+//    few column tiles to keep every SM loading, and the partial sums meet in
+//    distributed shared memory (in rank order; no workspace, no atomics).
+//  * w8a8_pair_kernel, many tokens: persistent, 256 x 256 tiles of a CTA pair
+//    (cta_group::2), two accumulators so that a tile's epilogue overlaps the
+//    next one's main loop. Gated: CTA 0 stages 128 gate channels and CTA 1 the
+//    same 128 up channels, so one MMA makes both halves and a row's epilogue
+//    thread holds gate and up of each of its 128 outputs.
+#include <type_traits>
 
 #include "pk_common.cuh"
 
 namespace pk {
 namespace {
 
+constexpr int kBK = 128;  // bytes of K per stage: one swizzle row
+constexpr int kKSteps = kBK / 32;
+constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 4;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+
 struct Params {
-  const uint8_t* a;
-  const uint8_t* w[2];
   const float* a_scale;
   const float* w_scale[2];
   const float* bias;
   void* out;
-  int64_t lda, ldw[2], ldo;
-  int64_t M;
-  int N, K;
+  int64_t ldo;
+  int M, N, K;
   int out_dtype, act;
+  int split;         // swap: CTAs per tile along K (the cluster)
+  int num_m, num_n;  // tiles
+  int whole;         // pair: units that are whole tiles; each later tile is two half-width units
+  int* status;
 };
 
-constexpr int kTile = 64, kBK = 64;
-
-__device__ __forceinline__ float gate(float g, int act) {
-  // g * sigmoid(t): SiLU with t = g, GELU's tanh form with t = 2 sqrt(2/pi) (g + 0.044715 g^3)
-  const float t = act == PK_ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return g / (1.0f + expf(-t));
+// kind::i8: D int32 (format 2), operands signed (1); kind::f8f6f4: D fp32, e4m3 (0)
+constexpr uint32_t idesc8(bool e4m3, int m, int n) {
+  return (e4m3 ? 1u << 4 : (2u << 4) | (1u << 7) | (1u << 10)) |
+         (static_cast<uint32_t>(n) >> 3 << 17) | (static_cast<uint32_t>(m) >> 4 << 24);
 }
 
-__device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float v) {
+template <bool kE4M3>
+__device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                      uint32_t acc) {
+  if constexpr (kE4M3) {
+    umma_f8(d, a, b, idesc, acc);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+
+template <bool kE4M3>
+__device__ __forceinline__ void umma8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t acc) {
+  if constexpr (kE4M3) {
+    umma_f8_pair(d, a, b, idesc, acc);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+
+// Named barrier over `nthreads` threads that tells each whether any said true.
+__device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.aligned.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
+
+template <bool kE4M3>
+__device__ __forceinline__ float acc_value(uint32_t raw) {
+  return kE4M3 ? __uint_as_float(raw) : static_cast<float>(static_cast<int>(raw));
+}
+
+// g * sigmoid(t): SiLU with t = g; GELU's tanh form with t = 2 sqrt(2/pi) (g +
+// 0.044715 g^3), since (1 + tanh(t/2)) / 2 = sigmoid(t).
+__device__ __forceinline__ float gated(float g, float u, int act) {
+  const float t = act == PK_ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+  return g / (1.0f + expf(-t)) * u;
+}
+
+__device__ __forceinline__ void store_one(void* out, int dtype, int64_t i, float v) {
   if (dtype == PK_F16)
     static_cast<__half*>(out)[i] = __float2half_rn(v);
   else
     store_elem(out, dtype, i, v);
 }
 
-template <bool kE4M3, bool kGated>
-__global__ void __launch_bounds__(256) w8a8_kernel(const Params p) {
-  constexpr int kW = kGated ? 2 : 1;
-  __shared__ uint32_t sa[kTile][kBK / 4 + 1], sw[kW][kTile][kBK / 4 + 1];
-  const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const int n0 = blockIdx.x * kTile;
-  int acc_i[kW][4][4] = {};
-  float acc_f[kW][4][4] = {};
+// Eight neighbouring outputs, `valid` of them inside the matrix.
+__device__ __forceinline__ void store_eight(void* out, int dtype, int64_t i, const float (&v)[8],
+                                            int valid) {
+  if (dtype == PK_F32) {
+    float* o = static_cast<float*>(out) + i;
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      return;
+    }
+  } else {
+    uint16_t* o = static_cast<uint16_t*>(out) + i;
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (dtype == PK_BF16) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        } else {
+          const __half2 p = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+      }
+      *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < valid) store_one(out, dtype, i + j, v[j]);
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: D[channel, token], one 128-channel x kNT-token tile per CTA.
+// ---------------------------------------------------------------------------
+template <int kNT, bool kGated>
+struct SwapCfg {
+  static constexpr int kW = kGated ? 2 : 1;                 // weight tiles per stage
+  static constexpr int kWTile = 128 * kBK;                  // 16 KB
+  static constexpr int kStageBytes = kW * kWTile + kNT * kBK;
+  // up to 64 tokens two CTAs share an SM when one weight is streamed
+  static constexpr int kBudget = !kGated && kNT <= 64 ? 110 * 1024 : 216 * 1024;
+  static constexpr int kStages = kBudget / kStageBytes;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kSmem = kBarOff + 256 + 1024;
+  static constexpr int kCols = kW * kNT;                    // accumulator columns
+  static constexpr int kTmem = kCols < 32 ? 32 : kCols;
+  static constexpr int kRedBytes = kCols * 128 * 4;         // partial sums of a K split
+  static constexpr bool kSplits = kRedBytes <= kBarOff;
+  static_assert(kSmem <= 227 * 1024 && kTmem <= 512, "one CTA fits an SM");
+};
+
+constexpr int kMaxSplit = 8;
+
+template <bool kE4M3, int kNT, bool kGated>
+__global__ void __launch_bounds__(kThreads)
+    w8a8_swap_kernel(const __grid_constant__ CUtensorMap tmA,
+                     const __grid_constant__ CUtensorMap tmW0,
+                     const __grid_constant__ CUtensorMap tmW1, const Params p) {
+  using C = SwapCfg<kNT, kGated>;
+  constexpr int kStages = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* empty = full + kStages;
+  uint64_t* done = empty + kStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // split fastest (the cluster), then the token tiles that share a weight tile
+  const int ks = static_cast<int>(blockIdx.x % p.split);
+  const int tile = static_cast<int>(blockIdx.x / p.split);
+  const int m0 = (tile % p.num_m) * kNT, n0 = (tile / p.num_m) * 128;
+  const int k_tiles = (p.K + kBK - 1) / kBK;
+  const int kt0 = static_cast<int>(static_cast<int64_t>(ks) * k_tiles / p.split);
+  const int kt1 = static_cast<int>(static_cast<int64_t>(ks + 1) * k_tiles / p.split);
+
+  if (warp == kTmaWarp && lane == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW0);
+    if (kGated) tma_prefetch_desc(&tmW1);
+    // the first weights start towards L2 while the previous kernel ends (a
+    // hint: nothing is read that it may still write)
+    for (int kt = kt0; kt < kt1 && kt < kt0 + kStages; ++kt) {
+      tma_prefetch_l2_2d(&tmW0, kt * kBK, n0);
+      if (kGated) tma_prefetch_l2_2d(&tmW1, kt * kBK, n0);
+    }
+  }
+  if (warp == kMmaWarp) tmem_alloc(tmem_holder, C::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
   griddep_wait();
   griddep_launch_dependents();
-  for (int k0 = 0; k0 < p.K; k0 += kBK) {
-    for (int i = t; i < kTile * (kBK / 4); i += 256) {
-      const int r = i / (kBK / 4), c = i % (kBK / 4);
-      auto word = [&](const uint8_t* base, int64_t row, int64_t rows, int64_t ld) {
-        uint32_t v = 0;
-        for (int b = 0; b < 4; ++b)
-          if (row < rows && k0 + 4 * c + b < p.K)
-            v |= static_cast<uint32_t>(base[row * ld + k0 + 4 * c + b]) << (8 * b);
-        return v;
-      };
-      sa[r][c] = word(p.a, m0 + r, p.M, p.lda);
-      for (int w = 0; w < kW; ++w) sw[w][r][c] = word(p.w[w], n0 + r, p.N, p.ldw[w]);
+
+  bool fail = false;
+  int issued = 0;
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      for (int kt = kt0, it = 0; kt < kt1; ++kt, ++it) {
+        const int st = it % kStages;
+        if (it >= kStages)
+          fail = !mbar_wait(&empty[st], ((it / kStages) - 1) & 1, p.status, kSiteW8SwapProducer);
+        if (fail) break;
+        uint8_t* base = smem + st * C::kStageBytes;
+        mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+        tma_load_2d(base, &tmW0, &full[st], kt * kBK, n0);
+        if (kGated) tma_load_2d(base + C::kWTile, &tmW1, &full[st], kt * kBK, n0);
+        tma_load_2d(base + C::kW * C::kWTile, &tmA, &full[st], kt * kBK, m0);
+        issued = it + 1;
+      }
     }
-    __syncthreads();
-    for (int c = 0; c < kBK / 4; ++c)
-      for (int w = 0; w < kW; ++w)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = sa[ty * 4 + i][c], y = sw[w][tx * 4 + j][c];
-            if (kE4M3) {
-              for (int b = 0; b < 4; ++b) {
-                const auto f = [](uint32_t v) {
-                  return __half2float(__half(__nv_cvt_fp8_to_halfraw(
-                      static_cast<__nv_fp8_storage_t>(v & 0xff), __NV_E4M3)));
-                };
-                acc_f[w][i][j] = fmaf(f(x >> (8 * b)), f(y >> (8 * b)), acc_f[w][i][j]);
-              }
-            } else {
-              acc_i[w][i][j] = __dp4a(static_cast<int>(x), static_cast<int>(y), acc_i[w][i][j]);
-            }
-          }
-    __syncthreads();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = idesc8(kE4M3, 128, kNT);
+      for (int kt = kt0, it = 0; kt < kt1; ++kt, ++it) {
+        const int st = it % kStages;
+        fail = !mbar_wait(&full[st], (it / kStages) & 1, p.status, kSiteW8SwapMma);
+        if (fail) break;
+        tc_fence_after();
+        const uint32_t w_base = smem_u32(smem + st * C::kStageBytes);
+        const uint32_t a_base = w_base + C::kW * C::kWTile;
+#pragma unroll
+        for (int s = 0; s < kKSteps; ++s) {
+          const uint64_t ad = make_smem_desc(a_base + s * 32, 16, 1024);
+#pragma unroll
+          for (int w = 0; w < C::kW; ++w)
+            umma8<kE4M3>(tmem + w * kNT, make_smem_desc(w_base + w * C::kWTile + s * 32, 16, 1024),
+                         ad, kIdesc, (it > 0 || s > 0) ? 1u : 0u);
+        }
+        umma_commit(&empty[st]);
+      }
+      if (!fail) umma_commit(done);
+    }
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i;
-      const int n = n0 + tx * 4 + j;
-      if (m >= p.M || n >= p.N) continue;
-      float v[kW];
-      for (int w = 0; w < kW; ++w)
-        v[w] = (kE4M3 ? acc_f[w][i][j] : static_cast<float>(acc_i[w][i][j])) * p.a_scale[m] *
-               p.w_scale[w][n];
-      float y = v[0];
-      if (kGated)
-        y = gate(v[0], p.act) * v[kW - 1];
-      else if (p.bias != nullptr)
-        y += p.bias[n];
-      store_out(p.out, p.out_dtype, m * p.ldo + n, y);
+
+  // ---- epilogue: a thread holds one channel, the columns are tokens ----
+  const int q = warp & 3;  // TMEM lane quarter this warp may access
+  const int nl = q * 32 + lane;
+  const int n = n0 + nl;
+  const int tokens = min(kNT, p.M - m0);
+  const bool epi = warp >= kEpiWarp0;
+  float sw[C::kW], bias = 0.0f;
+  if (epi) {
+#pragma unroll
+    for (int w = 0; w < C::kW; ++w) sw[w] = n < p.N ? p.w_scale[w][n] : 0.0f;
+    if (!kGated && p.bias != nullptr && n < p.N) bias = p.bias[n];
+    fail = !mbar_wait(done, 0, p.status, kSiteW8SwapEpilogue);
+    tc_fence_after();
+  }
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  auto emit = [&](int m, float x, float y) {  // x (and y): the token's sums for this channel
+    const float sa = p.a_scale[m0 + m];
+    x = x * sa * sw[0];
+    float v;
+    if constexpr (kGated)
+      v = gated(x, y * sa * sw[C::kW - 1], p.act);
+    else
+      v = p.bias != nullptr ? x + bias : x;
+    if (n < p.N) store_one(p.out, p.out_dtype, static_cast<int64_t>(m0 + m) * p.ldo + n, v);
+  };
+  if (p.split == 1) {
+    if (epi && !fail) {
+#pragma unroll 1
+      for (int c = 0; c < kNT && c < tokens; c += 16) {
+        uint32_t x[16], y[16];
+        tmem_ld_32x32b_x16(taddr + c, x);
+        if (kGated) tmem_ld_32x32b_x16(taddr + kNT + c, y);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c + i < tokens)
+            emit(c + i, acc_value<kE4M3>(x[i]), kGated ? acc_value<kE4M3>(y[i]) : 0.0f);
+      }
     }
+  } else if constexpr (C::kSplits) {
+    // Every CTA's sums into its own ring (drained: all its MMAs are done), then
+    // CTA r of the cluster adds up tokens r, r + split, .. over the ranks in
+    // order and stores them.
+    fail = __syncthreads_or(fail) != 0;
+    uint32_t* red = reinterpret_cast<uint32_t*>(smem);
+    if (epi && !fail) {
+#pragma unroll 1
+      for (int c = 0; c < C::kCols; c += 16) {
+        if (c % kNT >= tokens) continue;
+        uint32_t x[16];
+        tmem_ld_32x32b_x16(taddr + c, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) red[(c + i) * 128 + nl] = x[i];
+      }
+    }
+    cluster_sync();
+    if (epi && !fail) {
+      const uint32_t red_addr = smem_u32(red);
+      for (int m = ks; m < tokens; m += p.split) {
+        float sum[C::kW];
+#pragma unroll
+        for (int w = 0; w < C::kW; ++w) {
+          uint32_t x[kMaxSplit];
+#pragma unroll
+          for (int j = 0; j < kMaxSplit; ++j)
+            if (j < p.split)
+              x[j] = __float_as_uint(ld_cluster_f32(cluster_map(
+                  red_addr + ((w * kNT + m) * 128 + nl) * 4, static_cast<uint32_t>(j))));
+          if constexpr (kE4M3) {
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kMaxSplit; ++j)
+              if (j < p.split) s += __uint_as_float(x[j]);
+            sum[w] = s;
+          } else {
+            uint32_t s = 0;
+#pragma unroll
+            for (int j = 0; j < kMaxSplit; ++j)
+              if (j < p.split) s += x[j];
+            sum[w] = static_cast<float>(static_cast<int>(s));
+          }
+        }
+        emit(m, sum[0], sum[C::kW - 1]);
+      }
+    }
+    cluster_sync();  // no CTA leaves while another may read its sums
+  }
+
+  if (fail && warp == kTmaWarp && lane == 0) {
+    // copies already issued land before the CTA's shared memory is released
+    for (int s = 0; s < issued; ++s) mbar_wait(&full[s % kStages], (s / kStages) & 1, nullptr, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmem);
+}
+
+// ---------------------------------------------------------------------------
+// Many tokens: persistent CTA pairs, D[token, channel] tiles of 256 x 256
+// (gated: 256 tokens x 128 outputs, gate and up side by side).
+// ---------------------------------------------------------------------------
+struct PairCfg {
+  static constexpr int kATile = 128 * kBK;  // this CTA's 128 tokens
+  static constexpr int kBTile = 128 * kBK;  // this CTA's 128 channels, two boxes of 64
+  static constexpr int kBBox = 64 * kBK;
+  static constexpr int kStageBytes = kATile + kBTile;
+  static constexpr int kStages = 6;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kScaleOff = kBarOff + 256;           // [2][256] scales, [2][256] bias
+  static constexpr int kSmem = kScaleOff + 4 * 256 * 4 + 1024;
+  static constexpr int kAccCols = 256;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+constexpr int kGroupM = 8;
+
+// Unit u of the schedule: tile (tm, tn), and half -1 (whole), 0 or 1.
+__device__ __forceinline__ void pair_unit(int u, const Params& p, int& tm, int& tn, int& half) {
+  int t = u;
+  half = -1;
+  if (u >= p.whole) {
+    t = p.whole + ((u - p.whole) >> 1);
+    half = (u - p.whole) & 1;
+  }
+  // rows of tiles in groups, so that the tiles in flight share operands in L2
+  const int per_group = kGroupM * p.num_n;
+  const int g = t / per_group;
+  const int first = g * kGroupM;
+  const int gm = min(p.num_m - first, kGroupM);
+  tm = first + (t % per_group) % gm;
+  tn = (t % per_group) / gm;
+}
+
+template <bool kE4M3, bool kGated>
+__global__ void __launch_bounds__(kThreads, 1)
+    w8a8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+                     const __grid_constant__ CUtensorMap tmW0,
+                     const __grid_constant__ CUtensorMap tmW1, const Params p) {
+  using C = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* s_scale = reinterpret_cast<float*>(smem + C::kScaleOff);
+  float* s_bias = s_scale + 2 * 256;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int k_tiles = (p.K + kBK - 1) / kBK;
+  const int num_units = p.whole + 2 * (p.num_m * p.num_n - p.whole);
+  constexpr int kTileN = kGated ? 128 : 256;  // outputs of a tile
+
+  if (warp == kTmaWarp && lane == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * kEpiWarps);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW0);
+    if (kGated) tma_prefetch_desc(&tmW1);
+  }
+  if (warp == kMmaWarp) tmem_alloc_pair(tmem_holder, 512);
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  griddep_wait();
+
+  bool fail = false;
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      const CUtensorMap* tmW = kGated && rank == 1 ? &tmW1 : &tmW0;
+      const uint32_t full0 = cluster_map(smem_u32(&full[0]), 0);
+      int it = 0;
+      for (int u = pair; u < num_units && !fail; u += npairs) {
+        int tm, tn, half;
+        pair_unit(u, p, tm, tn, half);
+        const int row = tm * 256 + rank * 128;
+        // whole: 128 channels in two boxes; half: 64 of the half's outputs
+        const int boxes = half < 0 ? 2 : 1;
+        const int col = tn * kTileN + (kGated ? (half < 0 ? 0 : half * 64)
+                                              : (half < 0 ? rank * 128 : half * 128 + rank * 64));
+        const uint32_t tx = 2u * (C::kATile + boxes * C::kBBox);
+        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
+          const int st = it % C::kStages;
+          if (it >= C::kStages)
+            fail = !mbar_wait(&empty[st], ((it / C::kStages) - 1) & 1, p.status, kSiteW8PairProducer);
+          if (fail) break;
+          uint8_t* base = smem + st * C::kStageBytes;
+          const uint32_t bar = full0 + st * 8;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], tx);
+          tma_load_2d_pair(base, &tmA, bar, kt * kBK, row);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d_pair(base + C::kATile + b * C::kBBox, tmW, bar, kt * kBK, col + b * 64);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (rank == 0 && lane == 0) {
+      int it = 0, local = 0;
+      for (int u = pair; u < num_units && !fail; u += npairs, ++local) {
+        const uint32_t idesc = u < p.whole ? idesc8(kE4M3, 256, 256) : idesc8(kE4M3, 256, 128);
+        const int ab = local & 1;
+        if (local >= 2)
+          fail = !mbar_wait_cluster(&acc_empty[ab], ((local >> 1) - 1) & 1, p.status, kSiteW8PairMma);
+        if (fail) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem + ab * C::kAccCols;
+        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
+          const int st = it % C::kStages;
+          fail = !mbar_wait(&full[st], (it / C::kStages) & 1, p.status, kSiteW8PairMma);
+          if (fail) break;
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(smem + st * C::kStageBytes);
+#pragma unroll
+          for (int s = 0; s < kKSteps; ++s)
+            umma8_pair<kE4M3>(d_tmem, make_smem_desc(a_base + s * 32, 16, 1024),
+                              make_smem_desc(a_base + C::kATile + s * 32, 16, 1024), idesc,
+                              (kt > 0 || s > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[st]);
+        }
+        if (fail) break;
+        umma_commit_pair(&acc_full[ab]);
+      }
+    }
+  } else {
+    // ---- epilogue (both CTAs): a thread holds one token's row ----
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const int et = tid - kEpiWarp0 * 32;
+    const uint32_t acc_empty0 = cluster_map(smem_u32(&acc_empty[0]), 0);
+    int local = 0;
+    for (int u = pair; u < num_units && !fail; u += npairs, ++local) {
+      int tm, tn, half;
+      pair_unit(u, p, tm, tn, half);
+      const int ab = local & 1;
+      const int outs = half < 0 ? kTileN : kTileN / 2;  // outputs of this unit
+      const int n0 = tn * kTileN + (half > 0 ? kTileN / 2 : 0);
+      // this unit's channel scales (gate then up) and bias
+      float* sc = s_scale + ab * 256;
+      float* bs = s_bias + ab * 256;
+      for (int i = et; i < (kGated ? 2 * outs : outs); i += kEpiWarps * 32) {
+        const int w = kGated && i >= outs ? 1 : 0;
+        const int n = n0 + i - w * outs;
+        sc[i] = n < p.N ? p.w_scale[w][n] : 0.0f;
+        if (!kGated) bs[i] = p.bias != nullptr && n < p.N ? p.bias[n] : 0.0f;
+      }
+      const int row = tm * 256 + rank * 128 + q * 32 + lane;
+      const float sa = row < p.M ? p.a_scale[row] : 0.0f;
+      // one barrier a unit: the scales are in place, and the warps agree on
+      // whether the wait ran out (none is left waiting for one that gave up)
+      fail = named_bar_or(
+          1, kEpiWarps * 32,
+          !mbar_wait(&acc_full[ab], (local >> 1) & 1, p.status, kSiteW8PairEpilogue));
+      if (fail) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * C::kAccCols;
+#pragma unroll 1
+      for (int c = 0; c < outs; c += 32) {
+        uint32_t x[32], y[32];
+        tmem_ld_32x32b_x32(taddr + c, x);
+        if (kGated) tmem_ld_32x32b_x32(taddr + outs + c, y);
+        tmem_ld_wait();
+        if (row < p.M) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              v[e] = acc_value<kE4M3>(x[i + e]) * sa * sc[c + i + e];
+              if constexpr (kGated)
+                v[e] = gated(v[e], acc_value<kE4M3>(y[i + e]) * sa * sc[outs + c + i + e], p.act);
+              else if (p.bias != nullptr)
+                v[e] += bs[c + i + e];
+            }
+            const int n = n0 + c + i;
+            if (n < p.N)
+              store_eight(p.out, p.out_dtype, static_cast<int64_t>(row) * p.ldo + n, v, p.N - n);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty0 + ab * 8);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still touch its memory
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc_pair(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// launch
+// ---------------------------------------------------------------------------
+bool rows_map(CUtensorMap* m, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows,
+              const char** why) {
+  return encode_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, K, rows, ld, kBK, box_rows,
+                        CU_TENSOR_MAP_SWIZZLE_128B, why);
+}
+
+Params params_of(const W8A8Args& g) {
+  Params p{};
+  p.a_scale = g.a_scale;
+  p.w_scale[0] = g.w_scale[0];
+  p.w_scale[1] = g.w_scale[1];
+  p.bias = g.bias;
+  p.out = g.out;
+  p.ldo = g.ldo;
+  p.M = static_cast<int>(g.M);
+  p.N = static_cast<int>(g.N);
+  p.K = static_cast<int>(g.K);
+  p.out_dtype = g.out_dtype;
+  p.act = g.act;
+  p.split = 1;
+  p.status = g.status;
+  return p;
+}
+
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, int grid, int cluster, int smem, cudaStream_t s,
+                   const CUtensorMap (&tm)[3], const Params& p) {
+  cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, tm[0], tm[1], tm[2], p);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <bool kE4M3, int kNT, bool kGated>
+cudaError_t launch_swap(const W8A8Args& g, int split, cudaStream_t s, const char** why) {
+  using C = SwapCfg<kNT, kGated>;
+  CUtensorMap tm[3];
+  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, kNT, why) ||
+      !rows_map(&tm[1], g.w[0], g.N, g.K, g.ldw[0], 128, why))
+    return cudaErrorInvalidValue;
+  tm[2] = tm[1];
+  if (kGated && !rows_map(&tm[2], g.w[1], g.N, g.K, g.ldw[1], 128, why))
+    return cudaErrorInvalidValue;
+  Params p = params_of(g);
+  p.num_m = static_cast<int>(ceil_div(g.M, kNT));
+  p.num_n = static_cast<int>(ceil_div(g.N, 128));
+  p.split = C::kSplits ? split : 1;
+  const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;
+  if (grid >= (1ll << 31)) return cudaErrorInvalidConfiguration;
+  return launch(w8a8_swap_kernel<kE4M3, kNT, kGated>, static_cast<int>(grid), p.split, C::kSmem, s,
+                tm, p);
+}
+
+template <bool kE4M3, bool kGated>
+cudaError_t launch_swap_any(const W8A8Args& g, int nt, int split, cudaStream_t s,
+                            const char** why) {
+  switch (nt) {
+    case 16: return launch_swap<kE4M3, 16, kGated>(g, split, s, why);
+    case 32: return launch_swap<kE4M3, 32, kGated>(g, split, s, why);
+    case 64: return launch_swap<kE4M3, 64, kGated>(g, split, s, why);
+    case 128: return launch_swap<kE4M3, 128, kGated>(g, split, s, why);
+    default: return launch_swap<kE4M3, 256, kGated>(g, split, s, why);
+  }
+}
+
+template <bool kE4M3, bool kGated>
+cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
+  CUtensorMap tm[3];
+  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, 128, why) ||
+      !rows_map(&tm[1], g.w[0], g.N, g.K, g.ldw[0], 64, why))
+    return cudaErrorInvalidValue;
+  tm[2] = tm[1];
+  if (kGated && !rows_map(&tm[2], g.w[1], g.N, g.K, g.ldw[1], 64, why))
+    return cudaErrorInvalidValue;
+  Params p = params_of(g);
+  p.num_m = static_cast<int>(ceil_div(g.M, 256));
+  p.num_n = static_cast<int>(ceil_div(g.N, kGated ? 128 : 256));
+  const int tiles = p.num_m * p.num_n;
+  const int slots = num_sms() / 2;
+  // A partial last wave whose halves still fit one wave runs as half-width
+  // units: about half a tile's time instead of a whole one's.
+  p.whole = tiles;
+  const int tail = tiles % slots;
+  if (tiles > slots && tail > 0 && 2 * tail <= slots) p.whole = tiles - tail;
+  const int units = p.whole + 2 * (tiles - p.whole);
+  return launch(w8a8_pair_kernel<kE4M3, kGated>, 2 * (units < slots ? units : slots), 2,
+                PairCfg::kSmem, s, tm, p);
+}
+
+// Which kernel, how many tokens a tile, how many K splits: from the sizes alone.
+struct Plan {
+  bool pair;
+  int nt, split;
+};
+
+Plan plan_of(const W8A8Args& g) {
+  const int sms = num_sms();
+  Plan plan{false, 16, 1};
+  const int64_t pair_tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? 128 : 256);
+  if (g.M > 128 && pair_tiles >= sms / 2) {
+    plan.pair = true;
+    return plan;
+  }
+  while (plan.nt < 256 && plan.nt < g.M) plan.nt *= 2;
+  if (plan.nt > 128 && ceil_div(g.N, 128) * ceil_div(g.M, 256) < sms) plan.nt = 128;
+  const int64_t tiles = ceil_div(g.N, 128) * ceil_div(g.M, plan.nt);
+  const int64_t slots = !g.gated && plan.nt <= 64 ? 2 * sms : sms;
+  int64_t split = slots / tiles;
+  const int64_t k_tiles = ceil_div(g.K, kBK);
+  if (split > k_tiles) split = k_tiles;
+  if (split > kMaxSplit) split = kMaxSplit;
+  while (plan.split * 2 <= split) plan.split *= 2;
+  return plan;
+}
+
+template <bool kE4M3, bool kGated>
+cudaError_t launch_typed(const W8A8Args& g, cudaStream_t s, const char** why) {
+  const Plan plan = plan_of(g);
+  if (plan.pair) return launch_pair<kE4M3, kGated>(g, s, why);
+  return launch_swap_any<kE4M3, kGated>(g, plan.nt, plan.split, s, why);
 }
 
 }  // namespace
 
 cudaError_t launch_w8a8(const W8A8Args& g, cudaStream_t s, const char** why) {
-  (void)why;
-  Params p{};
-  p.a = static_cast<const uint8_t*>(g.a);
-  p.lda = g.lda;
-  p.a_scale = g.a_scale;
-  for (int i = 0; i < 2; ++i) {
-    p.w[i] = static_cast<const uint8_t*>(g.w[i]);
-    p.ldw[i] = g.ldw[i];
-    p.w_scale[i] = g.w_scale[i];
-  }
-  p.bias = g.bias;
-  p.out = g.out;
-  p.ldo = g.ldo;
-  p.M = g.M;
-  p.N = static_cast<int>(g.N);
-  p.K = static_cast<int>(g.K);
-  p.out_dtype = g.out_dtype;
-  p.act = g.act;
-  const dim3 grid(static_cast<unsigned>((g.N + kTile - 1) / kTile),
-                  static_cast<unsigned>((g.M + kTile - 1) / kTile));
-  if (g.gated) {
-    if (g.e4m3) w8a8_kernel<true, true><<<grid, 256, 0, s>>>(p);
-    else w8a8_kernel<false, true><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (g.e4m3) w8a8_kernel<true, false><<<grid, 256, 0, s>>>(p);
-    else w8a8_kernel<false, false><<<grid, 256, 0, s>>>(p);
-  }
-  return cudaGetLastError();
+  if (g.gated)
+    return g.e4m3 ? launch_typed<true, true>(g, s, why) : launch_typed<false, true>(g, s, why);
+  return g.e4m3 ? launch_typed<true, false>(g, s, why) : launch_typed<false, false>(g, s, why);
 }
 
 }  // namespace pk
