@@ -12,8 +12,8 @@
 // one reduction, not two (the sum for r, then the maximum of y): r multiplies
 // the whole row, so the codes of y are those of u_k = h_k * w_k, and the sum of
 // h^2 and the maximum of |u| are reduced together; r enters the scale alone.
-// The maximum is taken on the bit patterns of |u| (ordered like the values,
-// infinities and NaN on top), so a NaN cannot be lost in it.
+// The maximum propagates NaN (across threads on the bit patterns of |u|, ordered
+// like the values with infinities and NaN on top), so none can be lost in it.
 //
 // A row that holds a NaN or an infinity has no 8-bit form: it gets scale NaN
 // and codes 0, so that every product with it is NaN and no other row is
@@ -22,6 +22,8 @@
 // layer adds to, so the norm is that of the stored value) and the codes.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "pk_common.cuh"
 
 namespace pk {
@@ -29,8 +31,16 @@ namespace {
 
 constexpr float kTiny = 1e-12f;     // smallest row maximum, as in the int4 group scales
 constexpr uint32_t kInfBits = 0x7f800000u;
-// Threads of a CTA by chunks held: four or more need over 64 registers.
+// Threads of a CTA by chunks held, and the CTAs of an SM the registers are
+// kept to.
 constexpr int max_threads(int chunks) { return chunks >= 4 ? 512 : 1024; }
+#ifndef MINB4
+#define MINB4 2
+#endif
+#ifndef MINB8
+#define MINB8 2
+#endif
+constexpr int min_ctas(int chunks) { return chunks == 4 ? MINB4 : chunks == 8 ? MINB8 : 1; }
 constexpr int kRowWarps = 8;        // rows per CTA when a warp holds a row
 
 struct RowsParams {
@@ -72,20 +82,82 @@ __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ float as_type<float>(float v) { return v; }
 
-// Eight consecutive values, 16-byte accesses (two for fp32).
+// Eight consecutive values as they lie in memory: two of a 16-bit type stay in
+// one register until they are used (arrays of T made the compiler spread them
+// over eight, and a row of several chunks spilled).
 template <typename T>
-struct alignas(16) Eight {
-  T v[8];
+struct Eight {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void round(const float (&v)[8]) {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[j]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2 p = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
+  }
+
+  __device__ __forceinline__ T element(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
+    } else {
+      const uint16_t h = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+      return *reinterpret_cast<const T*>(&h);
+    }
+  }
 };
 
-template <typename T>
+// 16 bytes of a row (from L2: read once, and perhaps just written) or of the
+// norm's weights (kept in L1: every row of the SM reads them).
+template <bool kWeights>
+__device__ __forceinline__ uint4 load16(const uint4* p) {
+  return kWeights ? __ldg(p) : __ldcg(p);
+}
+
+// 16-byte accesses (two for fp32).
+template <typename T, bool kWeights>
 __device__ __forceinline__ Eight<T> load8(const T* p) {
   Eight<T> e;
-  uint4 w[sizeof(T) / 2];
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-    w[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
-  memcpy(&e, w, sizeof(e));
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+    const uint4 v = load16<kWeights>(reinterpret_cast<const uint4*>(p) + i);
+    e.w[4 * i] = v.x;
+    e.w[4 * i + 1] = v.y;
+    e.w[4 * i + 2] = v.z;
+    e.w[4 * i + 3] = v.w;
+  }
   return e;
 }
 
@@ -99,74 +171,80 @@ __device__ __forceinline__ void shift_words(const uint32_t (&in)[kWords + 4], in
 // load8 from an address that is aligned to its element only: the aligned
 // 16-byte blocks that hold the values (each holds at least one of them), and
 // a shift by the distance, which is the same for all chunks of a row.
-template <typename T>
+template <typename T, bool kWeights>
 __device__ __forceinline__ Eight<T> load8_shifted(const T* p) {
-  constexpr int kWords = sizeof(T) * 2;
+  constexpr int kWords = Eight<T>::kWords;
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
   const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
   uint32_t in[kWords + 4];
 #pragma unroll
   for (int i = 0; i < kWords / 4 + 1; ++i) {
-    const uint4 v = i < kWords / 4 || off != 0 ? __ldcg(base + i) : make_uint4(0, 0, 0, 0);
+    const uint4 v =
+        i < kWords / 4 || off != 0 ? load16<kWeights>(base + i) : make_uint4(0, 0, 0, 0);
     in[4 * i] = v.x;
     in[4 * i + 1] = v.y;
     in[4 * i + 2] = v.z;
     in[4 * i + 3] = v.w;
   }
   const int bits = (off & 3) * 8;
-  uint32_t out[kWords];
-  switch (off >> 2) {
-    case 0: shift_words<kWords, 0>(in, bits, out); break;
-    case 1: shift_words<kWords, 1>(in, bits, out); break;
-    case 2: shift_words<kWords, 2>(in, bits, out); break;
-    default: shift_words<kWords, 3>(in, bits, out); break;
-  }
   Eight<T> e;
-  memcpy(&e, out, sizeof(e));
+  switch (off >> 2) {
+    case 0: shift_words<kWords, 0>(in, bits, e.w); break;
+    case 1: shift_words<kWords, 1>(in, bits, e.w); break;
+    case 2: shift_words<kWords, 2>(in, bits, e.w); break;
+    default: shift_words<kWords, 3>(in, bits, e.w); break;
+  }
   return e;
 }
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const Eight<T>& e) {
-  uint4 w[sizeof(T) / 2];
-  memcpy(w, &e, sizeof(e));
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i)
+    reinterpret_cast<uint4*>(p)[i] =
+        make_uint4(e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2], e.w[4 * i + 3]);
 }
 
 // Columns c0 .. c0 + 7 of a row of `cols`, 0 past its end.
-template <typename T, bool kVec>
+template <typename T, bool kVec, bool kWeights = false>
 __device__ __forceinline__ Eight<T> load_row8(const T* row, int c0, int cols) {
-  if (c0 + 8 <= cols) return kVec ? load8<T>(row + c0) : load8_shifted<T>(row + c0);
+  if (c0 + 8 <= cols)
+    return kVec ? load8<T, kWeights>(row + c0) : load8_shifted<T, kWeights>(row + c0);
   Eight<T> e;
+  float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e.v[j] = c0 + j < cols ? row[c0 + j] : as_type<T>(0.0f);
+  for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? as_f32<T>(row[c0 + j]) : 0.0f;
+  e.round(v);  // the values themselves
   return e;
 }
 
-// Chunk at column c0 of the row's h in its own type. The first pass adds the
-// residual and stores the sum; a later one reads the thread's own stores.
+// The row's h at column c0 in its own type: x, or in a later pass over a row
+// with a residual the sum the thread itself has stored.
 template <typename T, bool kNorm, bool kVec>
-__device__ __forceinline__ Eight<T> load_chunk(const RowsParams& p, int64_t row, int c0,
-                                               bool first) {
-  const bool sum = kNorm && p.residual != nullptr;
-  if (sum && !first) return load_row8<T, kVec>(static_cast<const T*>(p.h) + row * p.ldh, c0, p.cols);
-  Eight<T> e = load_row8<T, kVec>(static_cast<const T*>(p.x) + row * p.ldx, c0, p.cols);
-  if (sum) {
-    const Eight<T> r =
-        load_row8<T, kVec>(static_cast<const T*>(p.residual) + row * p.ldr, c0, p.cols);
-    T* h = static_cast<T*>(p.h) + row * p.ldh + c0;
+__device__ __forceinline__ Eight<T> load_h(const RowsParams& p, int64_t row, int c0, bool first) {
+  if (kNorm && p.residual != nullptr && !first)
+    return load_row8<T, kVec>(static_cast<const T*>(p.h) + row * p.ldh, c0, p.cols);
+  return load_row8<T, kVec>(static_cast<const T*>(p.x) + row * p.ldx, c0, p.cols);
+}
+
+// h = x + residual, stored.
+template <typename T, bool kVec>
+__device__ __forceinline__ void add_residual(const RowsParams& p, int64_t row, int c0,
+                                             const Eight<T>& r, Eight<T>& e) {
+  T* h = static_cast<T*>(p.h) + row * p.ldh + c0;
+  float a[8], b[8];
+  e.values(a);
+  r.values(b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e.v[j] = as_type<T>(as_f32<T>(e.v[j]) + as_f32<T>(r.v[j]));
-    if (kVec && c0 + 8 <= p.cols) {
-      store8<T>(h, e);
-    } else {
+  for (int j = 0; j < 8; ++j) a[j] += b[j];
+  e.round(a);
+  if (kVec && c0 + 8 <= p.cols) {
+    store8<T>(h, e);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c0 + j < p.cols) h[j] = e.v[j];
-    }
+    for (int j = 0; j < 8; ++j)
+      if (c0 + j < p.cols) h[j] = e.element(j);
   }
-  return e;
 }
 
 // u = h * factor * weight of a chunk, the sum of (h * factor)^2 in `sum`. The
@@ -175,8 +253,7 @@ __device__ __forceinline__ Eight<T> load_chunk(const RowsParams& p, int64_t row,
 template <typename T, bool kNorm, bool kVec>
 __device__ __forceinline__ void values(const RowsParams& p, const Eight<T>& e, int c0,
                                        float factor, float (&u)[8], float& sum) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] = as_f32<T>(e.v[j]);
+  e.values(u);
   if constexpr (kNorm) {
     sum = 0.0f;
 #pragma unroll
@@ -184,20 +261,34 @@ __device__ __forceinline__ void values(const RowsParams& p, const Eight<T>& e, i
       u[j] *= factor;
       sum = fmaf(u[j], u[j], sum);
     }
-    if (p.weight_f32) {
-      const Eight<float> w = load_row8<float, kVec>(static_cast<const float*>(p.weight), c0, p.cols);
+    float w[8];
+    if (p.weight_f32)
+      load_row8<float, kVec, true>(static_cast<const float*>(p.weight), c0, p.cols).values(w);
+    else
+      load_row8<T, kVec, true>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] *= w.v[j];
-    } else {
-      const Eight<T> w = load_row8<T, kVec>(static_cast<const T*>(p.weight), c0, p.cols);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] *= as_f32<T>(w.v[j]);
-    }
+    for (int j = 0; j < 8; ++j) u[j] *= w[j];
   }
 }
 
-__device__ __forceinline__ uint32_t int8_code(float v) {
-  return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f))) & 0xffu;
+// Four int8 codes of u * f: adding 1.5 * 2^23 leaves the product, rounded half
+// to even by the addition (fused: one rounding), as an integer in the low bits.
+// |u * f| is at most 127 and a few last places, so no code passes 127. One
+// multiply-add a value and three byte selections, where conversions, clamps and
+// shifts took eight instructions.
+__device__ __forceinline__ uint32_t int8_codes4(const float* u, float f) {
+  constexpr float kMagic = 12582912.0f;
+  uint32_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(fmaf(u[j], f, kMagic));
+  return prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
+}
+
+// Largest of |a|, |b|, |c|; NaN if one is NaN.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
 }
 
 // Codes of the chunk at column c0. Rows of codes are 8-byte aligned on every
@@ -216,8 +307,7 @@ __device__ __forceinline__ void store_codes(const RowsParams& p, int64_t row, in
                                                    __NV_SATFINITE, __NV_E4M3);
       w[i] = lo | (hi << 16);
     } else {
-      w[i] = int8_code(u[4 * i] * f) | (int8_code(u[4 * i + 1] * f) << 8) |
-             (int8_code(u[4 * i + 2] * f) << 16) | (int8_code(u[4 * i + 3] * f) << 24);
+      w[i] = int8_codes4(u + 4 * i, f);
     }
   }
   if (p.codes_vec && c0 + 8 <= p.cols) {
@@ -246,7 +336,7 @@ constexpr int kBlocks = 128;  // sums of 256 columns in a held row (32768 column
 // 32 apart in order, those 32 sums by shuffles. So a row's codes and scale do
 // not depend on how many rows are with it, on strides or on alignment.
 template <typename T, bool kNorm, int kChunks, bool kVec>
-__global__ void __launch_bounds__(max_threads(kChunks)) rows8_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(max_threads(kChunks), min_ctas(kChunks)) rows8_kernel(const RowsParams p) {
   __shared__ float s_sum[kBlocks];
   __shared__ uint32_t s_max[32];
   const int lanes = p.lanes;
@@ -261,24 +351,43 @@ __global__ void __launch_bounds__(max_threads(kChunks)) rows8_kernel(const RowsP
   const int chunks = kChunks > 0 ? kChunks : (p.cols + lanes * 8 - 1) / (lanes * 8);
   Eight<T> held[kHeld];
   if constexpr (kChunks > 0) {
+    // every load of the row before its first store: h may be x or residual, so
+    // a store between them would hold the later loads back
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
-      held[c] = load_chunk<T, kNorm, kVec>(p, row, (c * lanes + t) * 8, true);
+      held[c] = load_h<T, kNorm, kVec>(p, row, (c * lanes + t) * 8, true);
+    if (kNorm && p.residual != nullptr) {
+      Eight<T> r[kHeld];
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        r[c] = load_row8<T, kVec>(static_cast<const T*>(p.residual) + row * p.ldr,
+                                  (c * lanes + t) * 8, p.cols);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        add_residual<T, kVec>(p, row, (c * lanes + t) * 8, r[c], held[c]);
+    }
   }
   float sum = 0.0f;
   uint32_t most = 0u;
   auto pass = [&](bool first, float factor) {
     float mine = 0.0f;  // one-warp rows: lane c holds block c; long rows: this warp's blocks
-    most = 0u;
+    float big = 0.0f;
     if (warps > 1) __syncthreads();  // an earlier pass has read s_sum
 #pragma unroll(kHeld)
     for (int c = 0; c < (kChunks > 0 ? kChunks : chunks); ++c) {
       const int c0 = (c * lanes + t) * 8;
-      if constexpr (kChunks == 0) held[0] = load_chunk<T, kNorm, kVec>(p, row, c0, first);
+      if constexpr (kChunks == 0) {
+        held[0] = load_h<T, kNorm, kVec>(p, row, c0, first);
+        if (kNorm && p.residual != nullptr && first)
+          add_residual<T, kVec>(
+              p, row, c0,
+              load_row8<T, kVec>(static_cast<const T*>(p.residual) + row * p.ldr, c0, p.cols),
+              held[0]);
+      }
       float u[8], s8 = 0.0f;
       values<T, kNorm, kVec>(p, held[kChunks > 0 ? c : 0], c0, factor, u, s8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(u[j]) & 0x7fffffffu);
+      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
       if constexpr (kNorm) {
         s8 = warp_sum(s8);
         if constexpr (kChunks == 0) {
@@ -290,7 +399,7 @@ __global__ void __launch_bounds__(max_threads(kChunks)) rows8_kernel(const RowsP
         }
       }
     }
-    most = __reduce_max_sync(0xffffffffu, most);
+    most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
     if (warps > 1) {
       if (lane == 0) {
         s_max[warp] = most;
@@ -326,7 +435,7 @@ __global__ void __launch_bounds__(max_threads(kChunks)) rows8_kernel(const RowsP
 #pragma unroll(kHeld)
   for (int c = 0; c < (kChunks > 0 ? kChunks : chunks); ++c) {
     const int c0 = (c * lanes + t) * 8;
-    if constexpr (kChunks == 0) held[0] = load_chunk<T, kNorm, kVec>(p, row, c0, false);
+    if constexpr (kChunks == 0) held[0] = load_h<T, kNorm, kVec>(p, row, c0, false);
     float u[8], unused;
     values<T, kNorm, kVec>(p, held[kChunks > 0 ? c : 0], c0, factor, u, unused);
     if (bad) {
@@ -337,40 +446,70 @@ __global__ void __launch_bounds__(max_threads(kChunks)) rows8_kernel(const RowsP
   }
 }
 
-// Sixteen codes a thread: one 16-byte load, 32 or 64 bytes of values.
-template <typename T, bool kVec>
+// Eight codes a thread: one 8-byte load, 16 or 32 bytes of values. Rows of
+// values that start off a 16-byte boundary (odd widths) begin with up to seven
+// single values (item 0), so that the chunks after them store whole; their
+// codes then start at any byte, and come from the two words that hold them.
+template <typename T>
 __global__ void __launch_bounds__(256)
     dequantize_rows_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                            const float* __restrict__ scale, T* __restrict__ out, int64_t ldo,
                            int64_t rows, int cols, int e4m3) {
   griddep_wait();
   griddep_launch_dependents();
-  auto value = [&](uint32_t code, float s) {
-    const float v =
-        e4m3 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code),
-                                                            __NV_E4M3)))
-             : static_cast<float>(static_cast<int8_t>(code));
-    return v * s;
-  };
-  const int c0 = (blockIdx.x * blockDim.x + threadIdx.x) * (kVec ? 16 : 1);
+  const int item = blockIdx.x * blockDim.x + threadIdx.x;
   for (int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; row < rows;
        row += static_cast<int64_t>(gridDim.y) * blockDim.y) {
     const uint8_t* src = q + row * ldq;
     T* dst = out + row * ldo;
     const float s = scale[row];
-    if (kVec && c0 + 16 <= cols) {
-      const uint4 w = __ldcg(reinterpret_cast<const uint4*>(src + c0));
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        Eight<T> v;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          v.v[j] = as_type<T>(value((words[2 * half + (j >> 2)] >> (8 * (j & 3))) & 0xffu, s));
-        store8<T>(dst + c0 + 8 * half, v);
+    const int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / sizeof(T));
+    const int c0 = head == 0 ? item * 8 : item == 0 ? 0 : head + (item - 1) * 8;
+    const int c1 = min(cols, head != 0 && item == 0 ? head : c0 + 8);
+    if (c0 >= c1) continue;
+    uint32_t w[2] = {0u, 0u};
+    if (c1 - c0 == 8) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src + c0);
+      const uint32_t* base = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+      const int bits = static_cast<int>(at & 3) * 8;
+      if ((at & 7) == 0) {
+        const uint2 v = __ldcg(reinterpret_cast<const uint2*>(at));
+        w[0] = v.x;
+        w[1] = v.y;
+      } else {
+        const uint32_t a = __ldcg(base), b = __ldcg(base + 1);
+        const uint32_t c = bits != 0 ? __ldcg(base + 2) : 0u;
+        w[0] = __funnelshift_r(a, b, bits);
+        w[1] = __funnelshift_r(b, c, bits);
       }
     } else {
-      for (int c = c0; c < min(c0 + (kVec ? 16 : 1), cols); ++c) dst[c] = as_type<T>(value(src[c], s));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j < c1) w[j >> 2] |= static_cast<uint32_t>(src[c0 + j]) << (8 * (j & 3));
+    }
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const uint32_t pair = w[j >> 2] >> (8 * (j & 2));
+      if (e4m3) {
+        const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair & 0xffffu),
+                                                   __NV_E4M3));
+        const float2 f = __half22float2(h);
+        v[j] = f.x * s;
+        v[j + 1] = f.y * s;
+      } else {
+        v[j] = static_cast<float>(static_cast<int8_t>(pair)) * s;
+        v[j + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8)) * s;
+      }
+    }
+    Eight<T> e;
+    e.round(v);
+    if (c1 - c0 == 8) {
+      store8<T>(dst + c0, e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j < c1) dst[c0 + j] = e.element(j);
     }
   }
 }
@@ -441,8 +580,7 @@ template <typename T>
 cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* scale, T* out,
                                     int64_t ldo, int64_t rows, int cols, int e4m3,
                                     cudaStream_t s) {
-  const bool vec = aligned16(q) && ldq % 16 == 0 && aligned16(out) && (ldo * sizeof(T)) % 16 == 0;
-  const int items = vec ? (cols + 15) / 16 : cols;
+  const int items = (cols + 7) / 8 + 1;  // one more for the start of an unaligned row
   int tx = 32;
   while (tx < 256 && tx < items) tx *= 2;
   const int ty = 256 / tx;
@@ -450,10 +588,8 @@ cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* 
   const dim3 grid(static_cast<unsigned>((items + tx - 1) / tx),
                   static_cast<unsigned>(gy < 65535 ? gy : 65535));
   const dim3 block(tx, ty);
-  return vec ? launch_chained(dequantize_rows_kernel<T, true>, grid, block, s, q, ldq, scale, out,
-                              ldo, rows, cols, e4m3)
-             : launch_chained(dequantize_rows_kernel<T, false>, grid, block, s, q, ldq, scale, out,
-                              ldo, rows, cols, e4m3);
+  return launch_chained(dequantize_rows_kernel<T>, grid, block, s, q, ldq, scale, out, ldo, rows,
+                        cols, e4m3);
 }
 
 }  // namespace
