@@ -22,6 +22,7 @@
 // layer adds to, so the norm is that of the stored value) and the codes.
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "pk_common.cuh"
@@ -31,17 +32,8 @@ namespace {
 
 constexpr float kTiny = 1e-12f;     // smallest row maximum, as in the int4 group scales
 constexpr uint32_t kInfBits = 0x7f800000u;
-// Threads of a CTA by chunks held, and the CTAs of an SM the registers are
-// kept to.
-constexpr int max_threads(int chunks) { return chunks >= 4 ? 512 : 1024; }
-#ifndef MINB4
-#define MINB4 2
-#endif
-#ifndef MINB8
-#define MINB8 2
-#endif
-constexpr int min_ctas(int chunks) { return chunks == 4 ? MINB4 : chunks == 8 ? MINB8 : 1; }
-constexpr int kRowWarps = 8;        // rows per CTA when a warp holds a row
+constexpr int kMaxLanes = 512;      // threads of a row
+constexpr int64_t kMostStaged = 225 * 1024;  // shared memory for rows in flight
 
 struct RowsParams {
   const void* x;
@@ -51,13 +43,17 @@ struct RowsParams {
   uint8_t* q;
   float* scale;
   int64_t ldx, ldr, ldh, ldq;
+  uint32_t sx, sr, sh, sq;  // the same in bytes
   int64_t rows;
   int cols;
   int lanes;             // threads of a row
+  int stages;            // rows in flight per group of threads
+  int slot;              // bytes of one staged row
   int weight_f32;
   int codes_vec;         // rows of codes 8-byte aligned
   int e4m3;
   float eps;
+  float inv_cols;
 };
 
 template <typename T>
@@ -168,6 +164,19 @@ __device__ __forceinline__ void shift_words(const uint32_t (&in)[kWords + 4], in
   for (int i = 0; i < kWords; ++i) out[i] = __funnelshift_r(in[i + kSkip], in[i + kSkip + 1], bits);
 }
 
+// kWords words from byte `off` of in[].
+template <int kWords>
+__device__ __forceinline__ void shift_any(const uint32_t (&in)[kWords + 4], int off,
+                                          uint32_t (&out)[kWords]) {
+  const int bits = (off & 3) * 8;
+  switch (off >> 2) {
+    case 0: shift_words<kWords, 0>(in, bits, out); break;
+    case 1: shift_words<kWords, 1>(in, bits, out); break;
+    case 2: shift_words<kWords, 2>(in, bits, out); break;
+    default: shift_words<kWords, 3>(in, bits, out); break;
+  }
+}
+
 // load8 from an address that is aligned to its element only: the aligned
 // 16-byte blocks that hold the values (each holds at least one of them), and
 // a shift by the distance, which is the same for all chunks of a row.
@@ -186,14 +195,8 @@ __device__ __forceinline__ Eight<T> load8_shifted(const T* p) {
     in[4 * i + 2] = v.z;
     in[4 * i + 3] = v.w;
   }
-  const int bits = (off & 3) * 8;
   Eight<T> e;
-  switch (off >> 2) {
-    case 0: shift_words<kWords, 0>(in, bits, e.w); break;
-    case 1: shift_words<kWords, 1>(in, bits, e.w); break;
-    case 2: shift_words<kWords, 2>(in, bits, e.w); break;
-    default: shift_words<kWords, 3>(in, bits, e.w); break;
-  }
+  shift_any<kWords>(in, off, e.w);
   return e;
 }
 
@@ -206,10 +209,11 @@ __device__ __forceinline__ void store8(T* p, const Eight<T>& e) {
 }
 
 // Columns c0 .. c0 + 7 of a row of `cols`, 0 past its end.
-template <typename T, bool kVec, bool kWeights = false>
+template <typename T, bool kWeights = false>
 __device__ __forceinline__ Eight<T> load_row8(const T* row, int c0, int cols) {
   if (c0 + 8 <= cols)
-    return kVec ? load8<T, kWeights>(row + c0) : load8_shifted<T, kWeights>(row + c0);
+    return (reinterpret_cast<uintptr_t>(row + c0) & 15) == 0 ? load8<T, kWeights>(row + c0)
+                                                             : load8_shifted<T, kWeights>(row + c0);
   Eight<T> e;
   float v[8];
 #pragma unroll
@@ -218,56 +222,32 @@ __device__ __forceinline__ Eight<T> load_row8(const T* row, int c0, int cols) {
   return e;
 }
 
-// The row's h at column c0 in its own type: x, or in a later pass over a row
-// with a residual the sum the thread itself has stored.
-template <typename T, bool kNorm, bool kVec>
-__device__ __forceinline__ Eight<T> load_h(const RowsParams& p, int64_t row, int c0, bool first) {
-  if (kNorm && p.residual != nullptr && !first)
-    return load_row8<T, kVec>(static_cast<const T*>(p.h) + row * p.ldh, c0, p.cols);
-  return load_row8<T, kVec>(static_cast<const T*>(p.x) + row * p.ldx, c0, p.cols);
+// Columns c0 .. c0 + 7 of the norm's weights; kWhole: aligned and whole.
+template <typename W, bool kWhole>
+__device__ __forceinline__ Eight<W> load_weights(const W* w, int c0, int cols) {
+  if constexpr (kWhole) return load8<W, true>(w + c0);
+  else return load_row8<W, true>(w, c0, cols);
 }
 
-// h = x + residual, stored.
-template <typename T, bool kVec>
-__device__ __forceinline__ void add_residual(const RowsParams& p, int64_t row, int c0,
-                                             const Eight<T>& r, Eight<T>& e) {
-  T* h = static_cast<T*>(p.h) + row * p.ldh + c0;
+// e + r, rounded to the stream's type.
+template <typename T>
+__device__ __forceinline__ void add(Eight<T>& e, const Eight<T>& r) {
   float a[8], b[8];
   e.values(a);
   r.values(b);
 #pragma unroll
   for (int j = 0; j < 8; ++j) a[j] += b[j];
   e.round(a);
-  if (kVec && c0 + 8 <= p.cols) {
-    store8<T>(h, e);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row8(T* row, int c0, int cols, const Eight<T>& e) {
+  if (c0 + 8 <= cols && (reinterpret_cast<uintptr_t>(row + c0) & 15) == 0) {
+    store8<T>(row + c0, e);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c0 + j < p.cols) h[j] = e.element(j);
-  }
-}
-
-// u = h * factor * weight of a chunk, the sum of (h * factor)^2 in `sum`. The
-// weights are read again for the codes (from L1 or L2) rather than u kept: a
-// held chunk is then 16 bytes a thread of a 16-bit type, not 32.
-template <typename T, bool kNorm, bool kVec>
-__device__ __forceinline__ void values(const RowsParams& p, const Eight<T>& e, int c0,
-                                       float factor, float (&u)[8], float& sum) {
-  e.values(u);
-  if constexpr (kNorm) {
-    sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u[j] *= factor;
-      sum = fmaf(u[j], u[j], sum);
-    }
-    float w[8];
-    if (p.weight_f32)
-      load_row8<float, kVec, true>(static_cast<const float*>(p.weight), c0, p.cols).values(w);
-    else
-      load_row8<T, kVec, true>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] *= w[j];
+      if (c0 + j < cols) row[c0 + j] = e.element(j);
   }
 }
 
@@ -291,31 +271,31 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   return r;
 }
 
-// Codes of the chunk at column c0. Rows of codes are 8-byte aligned on every
-// path the launcher calls vector; elsewhere (a caller's own pitch) by bytes.
-__device__ __forceinline__ void store_codes(const RowsParams& p, int64_t row, int c0,
-                                            const float (&u)[8], float f) {
-  uint8_t* q = p.q + row * p.ldq + c0;
-  const bool e4m3 = p.e4m3 != 0;
-  uint32_t w[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (e4m3) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(u[4 * i] * f, u[4 * i + 1] * f),
-                                                   __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(u[4 * i + 2] * f, u[4 * i + 3] * f),
-                                                   __NV_SATFINITE, __NV_E4M3);
-      w[i] = lo | (hi << 16);
-    } else {
-      w[i] = int8_codes4(u + 4 * i, f);
-    }
+template <bool kE4M3>
+__device__ __forceinline__ uint32_t codes4(const float* u, float f) {
+  if constexpr (kE4M3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(u[0] * f, u[1] * f), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(u[2] * f, u[3] * f), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    return prmt(lo, hi, 0x5410);
+  } else {
+    return int8_codes4(u, f);
   }
-  if (p.codes_vec && c0 + 8 <= p.cols) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+}
+
+// Codes of the chunk at column c0: whole where every chunk of the matrix is
+// (kWhole), else as the row's end and the caller's pitch allow.
+template <bool kE4M3, bool kWhole>
+__device__ __forceinline__ void store_codes(uint8_t* q, int c0, int cols, bool vec,
+                                            const float (&u)[8], float f) {
+  const uint32_t lo = codes4<kE4M3>(u, f), hi = codes4<kE4M3>(u + 4, f);
+  if (kWhole || (vec && c0 + 8 <= cols)) {
+    *reinterpret_cast<uint2*>(q + c0) = make_uint2(lo, hi);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c0 + j < p.cols) q[j] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
+      if (c0 + j < cols) q[c0 + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
   }
 }
 
@@ -326,131 +306,383 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-constexpr int kBlocks = 128;  // sums of 256 columns in a held row (32768 columns)
-
-// kChunks chunks of eight values per thread stay in registers; kChunks = 0
-// (rows of more than 32768 columns) reads the row again, from L2, instead.
-//
-// The sum is the same tree whatever the number of threads: eight columns in
-// order, 32 such chunks (a block of 256 columns) by a warp's shuffles, blocks
-// 32 apart in order, those 32 sums by shuffles. So a row's codes and scale do
-// not depend on how many rows are with it, on strides or on alignment.
-template <typename T, bool kNorm, int kChunks, bool kVec>
-__global__ void __launch_bounds__(max_threads(kChunks), min_ctas(kChunks)) rows8_kernel(const RowsParams p) {
-  __shared__ float s_sum[kBlocks];
-  __shared__ uint32_t s_max[32];
-  const int lanes = p.lanes;
-  const int t = threadIdx.x % lanes;
-  const int lane = threadIdx.x & 31, warps = lanes >> 5, warp = t >> 5;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
-  griddep_wait();
-  griddep_launch_dependents();
-  if (row >= p.rows) return;  // whole warps: a CTA with several rows has one per warp
-
-  constexpr int kHeld = kChunks > 0 ? kChunks : 1;
-  const int chunks = kChunks > 0 ? kChunks : (p.cols + lanes * 8 - 1) / (lanes * 8);
-  Eight<T> held[kHeld];
-  if constexpr (kChunks > 0) {
-    // every load of the row before its first store: h may be x or residual, so
-    // a store between them would hold the later loads back
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      held[c] = load_h<T, kNorm, kVec>(p, row, (c * lanes + t) * 8, true);
-    if (kNorm && p.residual != nullptr) {
-      Eight<T> r[kHeld];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        r[c] = load_row8<T, kVec>(static_cast<const T*>(p.residual) + row * p.ldr,
-                                  (c * lanes + t) * 8, p.cols);
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        add_residual<T, kVec>(p, row, (c * lanes + t) * 8, r[c], held[c]);
-    }
+// Sum of h^2 and largest |u| of a row over its threads, the same bits in each.
+// The order is fixed by the row's length (its number of threads), so a row's
+// codes and scale do not depend on how many rows are with it, on strides or on
+// alignment. `s_sum` and `s_max` alternate from call to call: one barrier each.
+template <bool kNorm>
+__device__ __forceinline__ void reduce_row(int lanes, float& sum, float big, uint32_t& most,
+                                           float* s_sum, uint32_t* s_max) {
+  if constexpr (kNorm) sum = warp_sum(sum);
+  most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+  if (lanes == 32) return;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x % lanes) >> 5, warps = lanes >> 5;
+  if (lane == 0) {
+    s_sum[warp] = sum;
+    s_max[warp] = most;
   }
-  float sum = 0.0f;
-  uint32_t most = 0u;
-  auto pass = [&](bool first, float factor) {
-    float mine = 0.0f;  // one-warp rows: lane c holds block c; long rows: this warp's blocks
-    float big = 0.0f;
-    if (warps > 1) __syncthreads();  // an earlier pass has read s_sum
-#pragma unroll(kHeld)
-    for (int c = 0; c < (kChunks > 0 ? kChunks : chunks); ++c) {
-      const int c0 = (c * lanes + t) * 8;
-      if constexpr (kChunks == 0) {
-        held[0] = load_h<T, kNorm, kVec>(p, row, c0, first);
-        if (kNorm && p.residual != nullptr && first)
-          add_residual<T, kVec>(
-              p, row, c0,
-              load_row8<T, kVec>(static_cast<const T*>(p.residual) + row * p.ldr, c0, p.cols),
-              held[0]);
-      }
-      float u[8], s8 = 0.0f;
-      values<T, kNorm, kVec>(p, held[kChunks > 0 ? c : 0], c0, factor, u, s8);
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
-      if constexpr (kNorm) {
-        s8 = warp_sum(s8);
-        if constexpr (kChunks == 0) {
-          mine += s8;
-        } else if (warps == 1) {
-          if (lane == c) mine = s8;
-        } else if (lane == 0) {
-          s_sum[c * warps + warp] = s8;
-        }
-      }
-    }
-    most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-    if (warps > 1) {
-      if (lane == 0) {
-        s_max[warp] = most;
-        if (kNorm && kChunks == 0) s_sum[warp] = mine;
-      }
-      __syncthreads();
-      most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[lane] : 0u);
-      if constexpr (kNorm) {
-        const int blocks = kHeld * warps;
-        mine = 0.0f;
-        for (int b = lane; b < blocks; b += 32) mine += s_sum[b];
-      }
-    }
-    if constexpr (kNorm) sum = warp_sum(mine);
-  };
-  pass(true, 1.0f);
-  float factor = 1.0f;
-  if (kNorm && (!(sum < __uint_as_float(kInfBits)) || most >= kInfBits)) {
-    // Magnitudes above ~1e19 square past fp32's range: once more on h * 2^-80,
-    // which cancels in the norm (eps does not reach such sums). A true
-    // infinity or NaN stays one.
-    factor = 8.271806125530277e-25f;  // 2^-80
-    pass(false, factor);
-  }
+  __syncthreads();
+  most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[lane] : 0u);
+  if constexpr (kNorm) sum = warp_sum(lane < warps ? s_sum[lane] : 0.0f);
+}
 
-  const float top = p.e4m3 ? 448.0f : 127.0f;
-  const float eps = factor == 1.0f ? p.eps : 0.0f;
-  const float r = kNorm ? 1.0f / sqrtf(sum / static_cast<float>(p.cols) + eps) : 1.0f;
+// A row from its reductions: its scale (stored by one thread) and the factor
+// that takes u to codes; 0 for a row that has no 8-bit form.
+constexpr float kDown = 8.271806125530277e-25f;  // 2^-80
+template <bool kNorm, bool kE4M3>
+__device__ __forceinline__ float finish_row(const RowsParams& p, int64_t row, float sum,
+                                            uint32_t most, bool scaled, bool store) {
+  // Every warp of the row does this, once a row: reciprocals by the special
+  // function unit (2 last places; __fdividef flushes nothing here, a is normal),
+  // the IEEE division only in the thread that stores the scale. With IEEE
+  // divisions throughout it cost as many instructions as a thread's values.
+  constexpr float top = kE4M3 ? 448.0f : 127.0f;
+  const float r = kNorm ? rsqrtf(fmaf(sum, p.inv_cols, scaled ? 0.0f : p.eps)) : 1.0f;
   const float a = fmaxf(__uint_as_float(most) * r, kTiny);
   const bool bad = most >= kInfBits || !(a < __uint_as_float(kInfBits)) || (kNorm && !(r > 0.0f));
-  const float f = kNorm ? r * (top / a) : top / a;
-  if (t == 0) p.scale[row] = bad ? __uint_as_float(0x7fc00000u) : a / top;
-#pragma unroll(kHeld)
-  for (int c = 0; c < (kChunks > 0 ? kChunks : chunks); ++c) {
-    const int c0 = (c * lanes + t) * 8;
-    if constexpr (kChunks == 0) held[0] = load_h<T, kNorm, kVec>(p, row, c0, false);
-    float u[8], unused;
-    values<T, kNorm, kVec>(p, held[kChunks > 0 ? c : 0], c0, factor, u, unused);
-    if (bad) {
+  if (store) p.scale[row] = bad ? __uint_as_float(0x7fc00000u) : a / top;
+  const float f = a < 1e36f ? __fdividef(top, a) : top / a;
+  return bad ? 0.0f : (kNorm ? r * f : f);
+}
+
+// Magnitudes above ~1e19 square past fp32's range, and a product with a weight
+// may pass it: such a row goes over its values once more as h * 2^-80, which
+// cancels in the norm (eps does not reach such sums). A true infinity or NaN
+// stays one.
+template <bool kNorm>
+__device__ __forceinline__ bool past_range(float sum, uint32_t most) {
+  return kNorm && (!(sum < __uint_as_float(kInfBits)) || most >= kInfBits);
+}
+
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void group_sync(int lanes) {
+  if (lanes == 32) __syncwarp();
+  else __syncthreads();
+}
+
+// The eight values at byte `at` of a staged row.
+template <typename T, bool kAligned>
+__device__ __forceinline__ Eight<T> staged8(uint32_t at) {
+  constexpr int kWords = Eight<T>::kWords;
+  Eight<T> e;
+  const int off = kAligned ? 0 : static_cast<int>(at & 15);
+  uint32_t in[kWords + 4];
+#pragma unroll
+  for (int i = 0; i < kWords / 4 + (kAligned ? 0 : 1); ++i) {
+    const uint4 v = lds_v4(at - off + 16 * i);
+    in[4 * i] = v.x;
+    in[4 * i + 1] = v.y;
+    in[4 * i + 2] = v.z;
+    in[4 * i + 3] = v.w;
+  }
+  if constexpr (kAligned) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) e.w[i] = in[i];
+  } else {
+    shift_any<kWords>(in, off, e.w);
+  }
+  return e;
+}
+
+enum Mode : int { kCodes = 0, kNormed = 1, kSummed = 2 };  // the quantizer; the norm without / with a residual
+
+constexpr int kHold = 4;  // chunks of a row a thread holds as fp32
+
+constexpr int kCtaThreads = 1024;  // threads an SM holds of it: 64 registers each
+
+// Rows staged in shared memory. A group of `lanes` threads walks its rows with
+// `stages` of them in flight (cp.async): a thread copies the chunks it will
+// read itself, so whole rows need no barrier but the reduction's; rows that
+// start off a 16-byte boundary are copied as the aligned blocks that hold them
+// (each holds at least one of their values) and shifted when they are read.
+// Between the passes a thread holds u of its chunks (kHeld; rows of up to 16384
+// columns), or the first pass leaves h in the slot for the second.
+//
+// kWhole: every row of every operand is whole 16-byte chunks. It is a
+// parameter of the kernel, not a test in it, because instructions set the
+// pace: with the tests inside, and h and the weights read twice, a value cost
+// 23 (codes) to 46 (norm with a residual) of them and the SMs issued at 70 % of
+// their rate (4096 x 8192 with a residual 54.9 us).
+template <typename T, Mode kMode, bool kE4M3, bool kWhole, bool kHeld>
+__global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_staged_kernel(const RowsParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_sum[2][32];
+  __shared__ uint32_t s_max[2][32];
+  constexpr bool kNorm = kMode != kCodes;
+  constexpr int kStreams = kMode == kSummed ? 2 : 1;
+  constexpr int kSize = sizeof(T);
+  const int lanes = p.lanes, groups = blockDim.x / lanes;
+  const int group = threadIdx.x / lanes, t = threadIdx.x % lanes;
+  // Rows and strides are 32 bits here (the launcher sees to it): an address is
+  // one wide multiply-add where it is needed, not a register pair kept for it.
+  const uint32_t step = gridDim.x * groups, first = blockIdx.x * groups + group;
+  const uint32_t rows = static_cast<uint32_t>(p.rows);
+  const uint32_t slots = smem_u32(smem) + group * p.stages * kStreams * p.slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  auto at = [](const void* base, uint32_t row, uint32_t stride) {
+    return static_cast<const uint8_t*>(base) + static_cast<uint64_t>(row) * stride;
+  };
+  // distance of a stream's row from its 16-byte block
+  auto offset = [&](const void* base, uint32_t row, uint32_t stride) {
+    return kWhole ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(at(base, row, stride)) & 15);
+  };
+  auto copy_row = [&](const uint8_t* src, uint32_t slot) {
+    const int bytes = p.cols * kSize;
+    if constexpr (kWhole) {
+      for (int b = t * 8 * kSize; b < bytes; b += lanes * 8 * kSize)
+#pragma unroll
+        for (int i = 0; i < kSize / 2; ++i) copy16_async(slot + b + 16 * i, src + b + 16 * i);
+    } else {
+      const int off = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 15);
+      for (int b = t * 16; b < off + bytes; b += lanes * 16) copy16_async(slot + b, src - off + b);
+    }
+  };
+  auto fetch = [&](uint32_t row, int stage) {
+    if (row < rows) {
+      const uint32_t slot = slots + stage * kStreams * p.slot;
+      copy_row(at(p.x, row, p.sx), slot);
+      if constexpr (kMode == kSummed) copy_row(at(p.residual, row, p.sr), slot + p.slot);
+    }
+    copy_commit();
+  };
+
+  for (int s = 0; s + 1 < p.stages; ++s) fetch(first + s * step, s);
+  if constexpr (kNorm) {  // the weights towards L1, where all rows of the SM read them
+    const int wsize = p.weight_f32 ? 4 : kSize;
+    for (int c0 = t * 8; c0 < p.cols; c0 += lanes * 8)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint8_t*>(p.weight) +
+                                                    static_cast<int64_t>(c0) * wsize));
+  }
+  int stage = 0, parity = 0;
+  // the same number of turns for every group of a CTA (a CTA has several only
+  // when each is a warp, whose reduction needs no barrier)
+  for (uint32_t base = blockIdx.x * groups; base < rows; base += step) {
+    const uint32_t row = base + group;
+    const bool live = row < rows;
+    fetch(row + (p.stages - 1) * step, stage == 0 ? p.stages - 1 : stage - 1);
+    if (p.stages == 2) copy_wait<1>();
+    else copy_wait<3>();
+    if constexpr (!kWhole) group_sync(lanes);
+    const uint32_t slot = slots + stage * kStreams * p.slot;
+    const int cols = live ? p.cols : 0;
+    const int off = offset(p.x, row, p.sx);
+    const int offr = kMode == kSummed ? offset(p.residual, row, p.sr) : 0;
+    T* h = reinterpret_cast<T*>(const_cast<uint8_t*>(at(p.h, row, p.sh)));
+    uint8_t* q = const_cast<uint8_t*>(at(p.q, row, p.sq));
+
+    // h of the chunk at c0. First: the residual's addition, h stored (and left in
+    // a whole row's slot where it is read again; another adds again).
+    auto chunk = [&](int c0, auto start) {
+      constexpr bool kStart = decltype(start)::value;
+      Eight<T> e = staged8<T, kWhole>(slot + off + c0 * kSize);
+      if constexpr (kMode == kSummed && (kStart || kHeld || !kWhole)) {
+        add<T>(e, staged8<T, kWhole>(slot + p.slot + offr + c0 * kSize));
+        if constexpr (kStart && kWhole) {
+          store8<T>(h + c0, e);
+          if constexpr (!kHeld) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::kWords / 4; ++i)
+              sts_v4u(slot + c0 * kSize + 16 * i, e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2],
+                      e.w[4 * i + 3]);
+          }
+        } else if constexpr (kStart) {
+          store_row8<T>(h, c0, p.cols, e);
+        }
+      }
+      return e;
+    };
+    // u = h * weight, the sum of h^2
+    auto values = [&](const Eight<T>& e, int c0, auto scaled, float (&u)[8], float& sum) {
+      e.values(u);
+      if (!kWhole && c0 + 8 > p.cols) {  // the row's last chunk
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = c0 + j < p.cols ? u[j] : 0.0f;
+      }
+      if constexpr (kNorm) {
+        float w[8];
+        if (p.weight_f32)
+          load_weights<float, kWhole>(static_cast<const float*>(p.weight), c0, p.cols).values(w);
+        else
+          load_weights<T, kWhole>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (decltype(scaled)::value) u[j] *= kDown;
+          sum = fmaf(u[j], u[j], sum);
+          u[j] *= w[j];
+        }
+      }
+    };
+    auto largest = [&](float big, const float (&u)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
+      return big;
+    };
+    auto put = [&](int c0, const float (&u)[8], float f) {
+      store_codes<kE4M3, kWhole>(q, c0, p.cols, p.codes_vec, u, f);
+    };
+    auto quantize = [&](auto scaled, float f) {  // from the staged row
+#pragma unroll 2
+      for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
+        float u[8] = {}, unused = 0.0f;
+        if (f != 0.0f) values(chunk(c0, std::false_type{}), c0, scaled, u, unused);
+        put(c0, u, f);
+      }
+    };
+
+    float sum = 0.0f, big = 0.0f;
+    uint32_t most;
+    float held[kHeld ? kHold : 1][8];
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int c = 0; c < kHold; ++c) {
+        const int c0 = (c * lanes + t) * 8;
+        if (c0 < cols) {
+          values(chunk(c0, std::true_type{}), c0, std::false_type{}, held[c], sum);
+          big = largest(big, held[c]);
+        }
+      }
+    } else {
+#pragma unroll 2
+      for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
+        values(chunk(c0, std::true_type{}), c0, std::false_type{}, held[0], sum);
+        big = largest(big, held[0]);
+      }
+    }
+    reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
+    parity ^= 1;
+    if (live && !past_range<kNorm>(sum, most)) {
+      const float f = finish_row<kNorm, kE4M3>(p, row, sum, most, false, t == 0);
+      if (!kHeld || f == 0.0f) {
+        quantize(std::false_type{}, f);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kHold; ++c) {
+          const int c0 = (c * lanes + t) * 8;
+          if (c0 < cols) put(c0, held[kHeld ? c : 0], f);
+        }
+      }
+    } else if (live) {  // the same for all threads of the row
+      sum = big = 0.0f;
+#pragma unroll 1
+      for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
+        values(chunk(c0, std::false_type{}), c0, std::true_type{}, held[0], sum);
+        big = largest(big, held[0]);
+      }
+      reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
+      parity ^= 1;
+      quantize(std::true_type{}, finish_row<kNorm, kE4M3>(p, row, sum, most, true, t == 0));
+    }
+    if constexpr (!kWhole) group_sync(lanes);  // the slot has been read by all
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+}
+
+// Rows too long for shared memory (or of which one alone would leave an SM with
+// nothing in flight): one CTA a row, read again, from L2, for the codes.
+template <typename T, bool kNorm, bool kE4M3>
+__global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams p) {
+  __shared__ float s_sum[2][32];
+  __shared__ uint32_t s_max[2][32];
+  const int64_t row = blockIdx.x;
+  const int t = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
+  T* h = static_cast<T*>(p.h) + row * p.ldh;
+  const bool residual = kNorm && p.residual != nullptr;
+  auto values = [&](bool start, float factor, int c0, float (&u)[8], float& sum) {
+    Eight<T> e = load_row8<T>(residual && !start ? h : x, c0, p.cols);
+    if (residual && start) {
+      add<T>(e, load_row8<T>(r, c0, p.cols));
+      store_row8<T>(h, c0, p.cols, e);
+    }
+    e.values(u);
+    if constexpr (kNorm) {
+      float w[8];
+      if (p.weight_f32)
+        load_row8<float, true>(static_cast<const float*>(p.weight), c0, p.cols).values(w);
+      else
+        load_row8<T, true>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[j] *= factor;
+        sum = fmaf(u[j], u[j], sum);
+        u[j] *= w[j];
+      }
+    }
+  };
+  float sum, factor = 1.0f;
+  uint32_t most;
+  auto pass = [&](bool start, int parity) {
+    float big = 0.0f;
+    sum = 0.0f;
+    for (int c0 = t * 8; c0 < p.cols; c0 += kMaxLanes * 8) {
+      float u[8];
+      values(start, factor, c0, u, sum);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
+    }
+    reduce_row<kNorm>(kMaxLanes, sum, big, most, s_sum[parity], s_max[parity]);
+  };
+  pass(true, 0);
+  const bool scaled = past_range<kNorm>(sum, most);
+  if (scaled) {
+    factor = kDown;
+    pass(false, 1);
+  }
+  const float f = finish_row<kNorm, kE4M3>(p, row, sum, most, scaled, t == 0);
+  for (int c0 = t * 8; c0 < p.cols; c0 += kMaxLanes * 8) {
+    float u[8], unused = 0.0f;
+    values(false, factor, c0, u, unused);
+    if (f == 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = 0.0f;
     }
-    store_codes(p, row, c0, u, bad ? 0.0f : f);
+    store_codes<kE4M3, false>(p.q + row * p.ldq, c0, p.cols, p.codes_vec, u, f);
   }
 }
 
-// Eight codes a thread: one 8-byte load, 16 or 32 bytes of values. Rows of
-// values that start off a 16-byte boundary (odd widths) begin with up to seven
-// single values (item 0), so that the chunks after them store whole; their
-// codes then start at any byte, and come from the two words that hold them.
+// Eight codes (two words) times the row's scale.
 template <typename T>
+__device__ __forceinline__ Eight<T> code_values(uint32_t w0, uint32_t w1, bool e4m3, float s) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const uint32_t pair = (j < 4 ? w0 : w1) >> (8 * (j & 2));
+    if (e4m3) {
+      const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair & 0xffffu),
+                                                 __NV_E4M3));
+      const float2 f = __half22float2(h);
+      v[j] = f.x * s;
+      v[j + 1] = f.y * s;
+    } else {
+      v[j] = static_cast<float>(static_cast<int8_t>(pair)) * s;
+      v[j + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8)) * s;
+    }
+  }
+  Eight<T> e;
+  e.round(v);
+  return e;
+}
+
+// kWhole: sixteen codes a thread, one 16-byte load (4096 x 8192 to bf16: 15.7
+// us, with eight 23.6). Else eight: rows of values that start off a 16-byte
+// boundary (odd widths) begin with up to seven single values (item 0), so that
+// the chunks after them store whole; their codes then start at any byte, and
+// come from the words that hold them (1000 x 5001: 5.7 us, by bytes 21.5).
+template <typename T, bool kWhole>
 __global__ void __launch_bounds__(256)
     dequantize_rows_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                            const float* __restrict__ scale, T* __restrict__ out, int64_t ldo,
@@ -462,48 +694,36 @@ __global__ void __launch_bounds__(256)
        row += static_cast<int64_t>(gridDim.y) * blockDim.y) {
     const uint8_t* src = q + row * ldq;
     T* dst = out + row * ldo;
-    const float s = scale[row];
-    const int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / sizeof(T));
+    if constexpr (kWhole) {
+      const int c0 = item * 16;
+      if (c0 >= cols) continue;
+      const float s = scale[row];
+      const uint4 w = __ldcg(reinterpret_cast<const uint4*>(src + c0));
+      store8<T>(dst + c0, code_values<T>(w.x, w.y, e4m3, s));
+      store8<T>(dst + c0 + 8, code_values<T>(w.z, w.w, e4m3, s));
+      continue;
+    }
+    const int head =
+        static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / sizeof(T));
     const int c0 = head == 0 ? item * 8 : item == 0 ? 0 : head + (item - 1) * 8;
     const int c1 = min(cols, head != 0 && item == 0 ? head : c0 + 8);
     if (c0 >= c1) continue;
+    const float s = scale[row];
     uint32_t w[2] = {0u, 0u};
     if (c1 - c0 == 8) {
       const uintptr_t at = reinterpret_cast<uintptr_t>(src + c0);
       const uint32_t* base = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
       const int bits = static_cast<int>(at & 3) * 8;
-      if ((at & 7) == 0) {
-        const uint2 v = __ldcg(reinterpret_cast<const uint2*>(at));
-        w[0] = v.x;
-        w[1] = v.y;
-      } else {
-        const uint32_t a = __ldcg(base), b = __ldcg(base + 1);
-        const uint32_t c = bits != 0 ? __ldcg(base + 2) : 0u;
-        w[0] = __funnelshift_r(a, b, bits);
-        w[1] = __funnelshift_r(b, c, bits);
-      }
+      const uint32_t a = __ldcg(base), b = __ldcg(base + 1);
+      const uint32_t c = bits != 0 ? __ldcg(base + 2) : 0u;
+      w[0] = __funnelshift_r(a, b, bits);
+      w[1] = __funnelshift_r(b, c, bits);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (c0 + j < c1) w[j >> 2] |= static_cast<uint32_t>(src[c0 + j]) << (8 * (j & 3));
     }
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const uint32_t pair = w[j >> 2] >> (8 * (j & 2));
-      if (e4m3) {
-        const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair & 0xffffu),
-                                                   __NV_E4M3));
-        const float2 f = __half22float2(h);
-        v[j] = f.x * s;
-        v[j + 1] = f.y * s;
-      } else {
-        v[j] = static_cast<float>(static_cast<int8_t>(pair)) * s;
-        v[j + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8)) * s;
-      }
-    }
-    Eight<T> e;
-    e.round(v);
+    const Eight<T> e = code_values<T>(w[0], w[1], e4m3, s);
     if (c1 - c0 == 8) {
       store8<T>(dst + c0, e);
     } else {
@@ -517,61 +737,96 @@ __global__ void __launch_bounds__(256)
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename... P, typename... A>
-cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t s, A... args) {
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t s,
+                           A... args) {
+  if (smem > 40 * 1024) {  // 48 KB less the static arrays need no attribute
+    const cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-// Threads per row and chunks per thread. A row of up to 1024 columns is one
-// warp's, eight rows to a CTA (no shared memory, no barrier); a longer row is a
-// CTA's. Few rows (decode) spread each row over as many threads as it has
-// chunks, for the shortest chain of loads.
-template <typename T, bool kNorm, bool kVec>
-cudaError_t launch_rows(RowsParams p, cudaStream_t s) {
-  const int items = (p.cols + 7) / 8;
-  const int per_lane = p.rows <= num_sms() ? 1 : 4;
-  int lanes = 32;
-  while (lanes < 1024 && lanes * per_lane < items) lanes *= 2;
-  if (items > 2 * 1024 && items <= 8 * 512) lanes = 512;
-  p.lanes = lanes;
-  const int chunks = (items + lanes - 1) / lanes;
-  const int threads = lanes == 32 ? 32 * kRowWarps : lanes;
-  const int64_t per_cta = threads / lanes;
-  const dim3 grid(static_cast<unsigned>((p.rows + per_cta - 1) / per_cta));
-  if (items > 8 * 512) return launch_chained(rows8_kernel<T, kNorm, 0, kVec>, grid, threads, s, p);
-  if (chunks <= 1) return launch_chained(rows8_kernel<T, kNorm, 1, kVec>, grid, threads, s, p);
-  if (chunks <= 2) return launch_chained(rows8_kernel<T, kNorm, 2, kVec>, grid, threads, s, p);
-  if (chunks <= 4) return launch_chained(rows8_kernel<T, kNorm, 4, kVec>, grid, threads, s, p);
-  return launch_chained(rows8_kernel<T, kNorm, 8, kVec>, grid, threads, s, p);
+template <typename T, Mode kMode, bool kE4M3>
+cudaError_t launch_staged(const RowsParams& p, bool whole, dim3 grid, int threads, int smem,
+                          cudaStream_t s) {
+  if (!whole)
+    return launch_chained(rows8_staged_kernel<T, kMode, kE4M3, false, true>, grid, threads, smem, s, p);
+  if (p.cols <= kHold * 8 * kMaxLanes)
+    return launch_chained(rows8_staged_kernel<T, kMode, kE4M3, true, true>, grid, threads, smem, s, p);
+  return launch_chained(rows8_staged_kernel<T, kMode, kE4M3, true, false>, grid, threads, smem, s, p);
 }
 
+template <typename T, bool kE4M3>
+cudaError_t launch_mode(const RowsParams& p, bool norm, bool whole, bool staged, int threads,
+                        int grid, int smem, cudaStream_t s) {
+  if (!staged)
+    return norm ? launch_chained(rows8_long_kernel<T, true, kE4M3>, grid, threads, 0, s, p)
+                : launch_chained(rows8_long_kernel<T, false, kE4M3>, grid, threads, 0, s, p);
+  if (!norm) return launch_staged<T, kCodes, kE4M3>(p, whole, grid, threads, smem, s);
+  return p.residual != nullptr ? launch_staged<T, kSummed, kE4M3>(p, whole, grid, threads, smem, s)
+                               : launch_staged<T, kNormed, kE4M3>(p, whole, grid, threads, smem, s);
+}
+
+// Threads per row: four chunks of eight columns each, up to kMaxLanes; a function
+// of the row's length alone (it fixes the order of the sum). With two chunks the
+// per-row work of twice as many warps costs more than it hides (8192 x 4096
+// codes 28.8 us, LANES4). Rows of up to 1024 columns are a warp's, several to a
+// CTA. Rows in flight: two, four of a warp's rows (short ones); the grid is what
+// fits the SMs at once.
 template <typename T>
-cudaError_t launch_rows_typed(RowsParams p, bool norm, cudaStream_t s) {
-  const auto whole = [](const void* b, int64_t ld, int64_t size) {
-    return aligned16(b) && (ld * size) % 16 == 0;
+cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
+  constexpr int kSize = sizeof(T);
+  p.lanes = 32;
+  while (p.lanes < kMaxLanes && p.lanes * 32 < p.cols) p.lanes *= 2;
+  p.inv_cols = 1.0f / static_cast<float>(p.cols);
+  const bool residual = norm && p.residual != nullptr;
+  const auto whole = [](const void* b, int64_t ld) {
+    return aligned16(b) && (ld * kSize) % 16 == 0;
   };
-  const bool vec = whole(p.x, p.ldx, sizeof(T)) &&
-                   (p.residual == nullptr ||
-                    (whole(p.residual, p.ldr, sizeof(T)) && whole(p.h, p.ldh, sizeof(T)))) &&
-                   (!norm || aligned16(p.weight));
   p.codes_vec = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0;
-  if (norm) return vec ? launch_rows<T, true, true>(p, s) : launch_rows<T, true, false>(p, s);
-  return vec ? launch_rows<T, false, true>(p, s) : launch_rows<T, false, false>(p, s);
+  const bool chunks = p.cols % 8 == 0 && p.codes_vec && whole(p.x, p.ldx) &&
+                      (!residual || (whole(p.residual, p.ldr) && whole(p.h, p.ldh))) &&
+                      (!norm || aligned16(p.weight));
+
+  const int threads = p.lanes == 32 ? 128 : p.lanes;
+  const int groups = threads / p.lanes;
+  // a chunk past an unaligned row's last block is read (and discarded)
+  const int64_t cols8 = static_cast<int64_t>(p.cols + 7) / 8 * 8;
+  const int64_t slot = cols8 * kSize + (chunks ? 0 : 32);
+  p.stages = p.lanes == 32 ? 4 : 2;
+  const int64_t bytes = slot * (residual ? 2 : 1) * groups * p.stages;
+  const int64_t widest = std::max({p.ldx, p.ldr, p.ldh, p.ldq}) * kSize;
+  p.sx = static_cast<uint32_t>(p.ldx * kSize);
+  p.sr = static_cast<uint32_t>(p.ldr * kSize);
+  p.sh = static_cast<uint32_t>(p.ldh * kSize);
+  p.sq = static_cast<uint32_t>(p.ldq);
+  const bool staged = bytes <= kMostStaged && widest < (1ll << 32) && (chunks || p.cols <= kHold * 8 * kMaxLanes);
+  p.slot = static_cast<int>(staged ? slot : 0);
+  const int64_t per_sm = std::max<int64_t>(
+      1, std::min<int64_t>(kCtaThreads / threads, 228 * 1024 / (bytes + 1536)));
+  const int64_t ctas = (p.rows + groups - 1) / groups;
+  const int grid =
+      static_cast<int>(staged ? std::min<int64_t>(ctas, per_sm * num_sms()) : p.rows);
+  const int smem = static_cast<int>(staged ? bytes : 0);
+  return p.e4m3 ? launch_mode<T, true>(p, norm, chunks, staged, threads, grid, smem, s)
+                : launch_mode<T, false>(p, norm, chunks, staged, threads, grid, smem, s);
 }
 
 cudaError_t launch_rows_any(const RowsParams& p, int dtype, bool norm, cudaStream_t s) {
   switch (dtype) {
-    case PK_F16: return launch_rows_typed<__half>(p, norm, s);
-    case PK_BF16: return launch_rows_typed<__nv_bfloat16>(p, norm, s);
-    case PK_F32: return launch_rows_typed<float>(p, norm, s);
+    case PK_F16: return launch_rows<__half>(p, norm, s);
+    case PK_BF16: return launch_rows<__nv_bfloat16>(p, norm, s);
+    case PK_F32: return launch_rows<float>(p, norm, s);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -580,7 +835,10 @@ template <typename T>
 cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* scale, T* out,
                                     int64_t ldo, int64_t rows, int cols, int e4m3,
                                     cudaStream_t s) {
-  const int items = (cols + 7) / 8 + 1;  // one more for the start of an unaligned row
+  const bool whole = cols % 16 == 0 && aligned16(q) && ldq % 16 == 0 && aligned16(out) &&
+                     (ldo * sizeof(T)) % 16 == 0;
+  // one item more for the start of an unaligned row
+  const int items = whole ? cols / 16 : (cols + 7) / 8 + 1;
   int tx = 32;
   while (tx < 256 && tx < items) tx *= 2;
   const int ty = 256 / tx;
@@ -588,8 +846,10 @@ cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* 
   const dim3 grid(static_cast<unsigned>((items + tx - 1) / tx),
                   static_cast<unsigned>(gy < 65535 ? gy : 65535));
   const dim3 block(tx, ty);
-  return launch_chained(dequantize_rows_kernel<T>, grid, block, s, q, ldq, scale, out, ldo, rows,
-                        cols, e4m3);
+  return whole ? launch_chained(dequantize_rows_kernel<T, true>, grid, block, 0, s, q, ldq, scale,
+                                out, ldo, rows, cols, e4m3)
+               : launch_chained(dequantize_rows_kernel<T, false>, grid, block, 0, s, q, ldq, scale,
+                                out, ldo, rows, cols, e4m3);
 }
 
 }  // namespace
