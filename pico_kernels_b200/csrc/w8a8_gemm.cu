@@ -29,6 +29,8 @@ constexpr int kBK = 128;  // bytes of K per stage: one swizzle row
 constexpr int kKSteps = kBK / 32;
 constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 4;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr int kPairEpiWarps = 8;  // two per TMEM lane quarter, half the columns each
+constexpr int kPairThreads = (kEpiWarp0 + kPairEpiWarps) * 32;
 
 struct Params {
   const float* a_scale;
@@ -100,10 +102,14 @@ __device__ __forceinline__ float acc_value(uint32_t raw) {
 }
 
 // g * sigmoid(t): SiLU with t = g; GELU's tanh form with t = 2 sqrt(2/pi) (g +
-// 0.044715 g^3), since (1 + tanh(t/2)) / 2 = sigmoid(t).
+// 0.044715 g^3), since (1 + tanh(t/2)) / 2 = sigmoid(t). The fast exponential
+// and quotient are off by about |t| + 6 last places where t < 0 (in the tail,
+// where the result vanishes) and by a few elsewhere; expf and an IEEE division
+// made the epilogue of a 256 x 128 tile longer than its main loop (4096 x 11008
+// x 4096: 362 us).
 __device__ __forceinline__ float gated(float g, float u, int act) {
   const float t = act == PK_ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return g / (1.0f + expf(-t)) * u;
+  return __fdividef(g, 1.0f + __expf(-t)) * u;
 }
 
 __device__ __forceinline__ void store_one(void* out, int dtype, int64_t i, float v) {
@@ -393,7 +399,7 @@ __device__ __forceinline__ void pair_unit(int u, const Params& p, int& tm, int& 
 }
 
 template <bool kE4M3, bool kGated>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     w8a8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmW0,
                      const __grid_constant__ CUtensorMap tmW1, const Params p) {
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 2 * kEpiWarps);
+      mbar_init(&acc_empty[i], 2 * kPairEpiWarps);
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
@@ -497,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- epilogue (both CTAs): a thread holds one token's row ----
     const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const int part = (warp - kEpiWarp0) >> 2;  // which half of the unit's outputs
     const int et = tid - kEpiWarp0 * 32;
     const uint32_t acc_empty0 = cluster_map(smem_u32(&acc_empty[0]), 0);
     int local = 0;
@@ -509,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // this unit's channel scales (gate then up) and bias
       float* sc = s_scale + ab * 256;
       float* bs = s_bias + ab * 256;
-      for (int i = et; i < (kGated ? 2 * outs : outs); i += kEpiWarps * 32) {
+      for (int i = et; i < (kGated ? 2 * outs : outs); i += kPairEpiWarps * 32) {
         const int w = kGated && i >= outs ? 1 : 0;
         const int n = n0 + i - w * outs;
         sc[i] = n < p.N ? p.w_scale[w][n] : 0.0f;
@@ -520,13 +527,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // one barrier a unit: the scales are in place, and the warps agree on
       // whether the wait ran out (none is left waiting for one that gave up)
       fail = named_bar_or(
-          1, kEpiWarps * 32,
+          1, kPairEpiWarps * 32,
           !mbar_wait(&acc_full[ab], (local >> 1) & 1, p.status, kSiteW8PairEpilogue));
       if (fail) break;
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * C::kAccCols;
 #pragma unroll 1
-      for (int c = 0; c < outs; c += 32) {
+      for (int c = part * (outs / 2); c < (part + 1) * (outs / 2); c += 32) {
         uint32_t x[32], y[32];
         tmem_ld_32x32b_x32(taddr + c, x);
         if (kGated) tmem_ld_32x32b_x32(taddr + outs + c, y);
@@ -590,7 +597,7 @@ Params params_of(const W8A8Args& g) {
 }
 
 template <typename Kernel>
-cudaError_t launch(Kernel kernel, int grid, int cluster, int smem, cudaStream_t s,
+cudaError_t launch(Kernel kernel, int grid, int threads, int cluster, int smem, cudaStream_t s,
                    const CUtensorMap (&tm)[3], const Params& p) {
   cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
@@ -603,7 +610,7 @@ cudaError_t launch(Kernel kernel, int grid, int cluster, int smem, cudaStream_t 
   attrs[1].val.clusterDim.y = 1;
   attrs[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attrs;
@@ -629,8 +636,8 @@ cudaError_t launch_swap(const W8A8Args& g, int split, cudaStream_t s, const char
   p.split = C::kSplits ? split : 1;
   const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;
   if (grid >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-  return launch(w8a8_swap_kernel<kE4M3, kNT, kGated>, static_cast<int>(grid), p.split, C::kSmem, s,
-                tm, p);
+  return launch(w8a8_swap_kernel<kE4M3, kNT, kGated>, static_cast<int>(grid), kThreads, p.split,
+                C::kSmem, s, tm, p);
 }
 
 template <bool kE4M3, bool kGated>
@@ -665,8 +672,8 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
   const int tail = tiles % slots;
   if (tiles > slots && tail > 0 && 2 * tail <= slots) p.whole = tiles - tail;
   const int units = p.whole + 2 * (tiles - p.whole);
-  return launch(w8a8_pair_kernel<kE4M3, kGated>, 2 * (units < slots ? units : slots), 2,
-                PairCfg::kSmem, s, tm, p);
+  return launch(w8a8_pair_kernel<kE4M3, kGated>, 2 * (units < slots ? units : slots),
+                kPairThreads, 2, PairCfg::kSmem, s, tm, p);
 }
 
 // Which kernel, how many tokens a tile, how many K splits: from the sizes alone.
