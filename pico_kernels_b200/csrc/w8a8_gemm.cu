@@ -27,10 +27,10 @@ namespace {
 
 constexpr int kBK = 128;  // bytes of K per stage: one swizzle row
 constexpr int kKSteps = kBK / 32;
-constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 4;
-constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
-constexpr int kPairEpiWarps = 8;  // two per TMEM lane quarter, half the columns each
-constexpr int kPairThreads = (kEpiWarp0 + kPairEpiWarps) * 32;
+constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2;
+constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, half the columns each
+constexpr int kEpiThreads = kEpiWarps * 32;
+constexpr int kThreads = kEpiWarp0 * 32 + kEpiThreads;
 
 struct Params {
   const float* a_scale;
@@ -40,6 +40,7 @@ struct Params {
   int64_t ldo;
   int M, N, K;
   int out_dtype, act;
+  int rows16;        // the output's rows start on 16-byte boundaries
   int split;         // swap: CTAs per tile along K (the cluster)
   int num_m, num_n;  // tiles
   int whole;         // pair: units that are whole tiles; each later tile is two half-width units
@@ -112,26 +113,43 @@ __device__ __forceinline__ float gated(float g, float u, int act) {
   return __fdividef(g, 1.0f + __expf(-t)) * u;
 }
 
+__device__ __forceinline__ void put(float* o, float v) { *o = v; }
+__device__ __forceinline__ void put(__half* o, float v) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
+
 __device__ __forceinline__ void store_one(void* out, int dtype, int64_t i, float v) {
   if (dtype == PK_F16)
-    static_cast<__half*>(out)[i] = __float2half_rn(v);
+    put(static_cast<__half*>(out) + i, v);
   else
     store_elem(out, dtype, i, v);
 }
 
-// Eight neighbouring outputs, `valid` of them inside the matrix.
+// f(the output as its own type)
+template <typename F>
+__device__ __forceinline__ void with_type(void* out, int dtype, F f) {
+  if (dtype == PK_F32) f(static_cast<float*>(out));
+  else if (dtype == PK_BF16) f(static_cast<__nv_bfloat16*>(out));
+  else f(static_cast<__half*>(out));
+}
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Eight neighbouring outputs from a 16-byte boundary on, `valid` of them inside
+// the matrix.
 __device__ __forceinline__ void store_eight(void* out, int dtype, int64_t i, const float (&v)[8],
                                             int valid) {
   if (dtype == PK_F32) {
     float* o = static_cast<float*>(out) + i;
-    if (valid >= 8 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+    if (valid >= 8) {
       reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
       return;
     }
   } else {
     uint16_t* o = static_cast<uint16_t*>(out) + i;
-    if (valid >= 8 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+    if (valid >= 8) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -162,13 +180,17 @@ struct SwapCfg {
   static constexpr int kStageBytes = kW * kWTile + kNT * kBK;
   // up to 64 tokens two CTAs share an SM when one weight is streamed
   static constexpr int kBudget = !kGated && kNT <= 64 ? 110 * 1024 : 216 * 1024;
-  static constexpr int kStages = kBudget / kStageBytes;
-  static constexpr int kBarOff = kStages * kStageBytes;
-  static constexpr int kSmem = kBarOff + 256 + 1024;
   static constexpr int kCols = kW * kNT;                    // accumulator columns
   static constexpr int kTmem = kCols < 32 ? 32 : kCols;
-  static constexpr int kRedBytes = kCols * 128 * 4;         // partial sums of a K split
-  static constexpr bool kSplits = kRedBytes <= kBarOff;
+  // partial sums of a K split: their own memory when small, else the drained ring
+  static constexpr int kRedBytes = kCols * 128 * 4;
+  static constexpr bool kOwnRed = kRedBytes <= 16 * 1024;
+  static constexpr int kStages = (kBudget - (kOwnRed ? kRedBytes : 0)) / kStageBytes;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kScaleOff = kBarOff + 256;
+  static constexpr int kRedOff = kOwnRed ? kScaleOff + kNT * 4 : 0;
+  static constexpr int kSmem = kScaleOff + kNT * 4 + (kOwnRed ? kRedBytes : 0) + 1024;
+  static constexpr bool kSplits = kOwnRed || kRedBytes <= kBarOff;
   static_assert(kSmem <= 227 * 1024 && kTmem <= 512, "one CTA fits an SM");
 };
 
@@ -220,6 +242,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  // a CTA's own memory for sums takes them from a CTA that has started
+  if (C::kOwnRed && p.split > 1) cluster_sync();
   griddep_wait();
   griddep_launch_dependents();
 
@@ -267,90 +291,113 @@ __global__ void __launch_bounds__(kThreads)
   // ---- epilogue: a thread holds one channel, the columns are tokens ----
   const int q = warp & 3;  // TMEM lane quarter this warp may access
   const int nl = q * 32 + lane;
-  const int n = n0 + nl;
   const int tokens = min(kNT, p.M - m0);
   const bool epi = warp >= kEpiWarp0;
+  const int part = (warp - kEpiWarp0) >> 2;  // which half of the tokens (epilogue warps)
+  float* s_sa = reinterpret_cast<float*>(smem + C::kScaleOff);
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  // this thread's channel and what its epilogue multiplies and adds
+  const int et = tid - kEpiWarp0 * 32;
+  const int ch = p.split == 1 ? nl : et & 127;
+  const int n = n0 + ch;
+  const bool inside = epi && n < p.N;
+  const bool biased = !kGated && p.bias != nullptr;
   float sw[C::kW], bias = 0.0f;
+  auto finish = [&](int m, float x, float y) {
+    const float sa = s_sa[m];
+    x = x * sa * sw[0];
+    if constexpr (kGated) return gated(x, y * sa * sw[C::kW - 1], p.act);
+    return biased ? x + bias : x;
+  };
   if (epi) {
 #pragma unroll
-    for (int w = 0; w < C::kW; ++w) sw[w] = n < p.N ? p.w_scale[w][n] : 0.0f;
-    if (!kGated && p.bias != nullptr && n < p.N) bias = p.bias[n];
-    fail = !mbar_wait(done, 0, p.status, kSiteW8SwapEpilogue);
+    for (int w = 0; w < C::kW; ++w) sw[w] = inside ? p.w_scale[w][n] : 0.0f;
+    if (biased && inside) bias = p.bias[n];
+    for (int m = et; m < tokens; m += kEpiThreads) s_sa[m] = p.a_scale[m0 + m];
+    named_bar_sync(1, kEpiThreads);
+    // a warp gives up as one (its TMEM loads are collective)
+    fail = __any_sync(0xffffffffu, !mbar_wait(done, 0, p.status, kSiteW8SwapEpilogue));
     tc_fence_after();
   }
-  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
-  auto emit = [&](int m, float x, float y) {  // x (and y): the token's sums for this channel
-    const float sa = p.a_scale[m0 + m];
-    x = x * sa * sw[0];
-    float v;
-    if constexpr (kGated)
-      v = gated(x, y * sa * sw[C::kW - 1], p.act);
-    else
-      v = p.bias != nullptr ? x + bias : x;
-    if (n < p.N) store_one(p.out, p.out_dtype, static_cast<int64_t>(m0 + m) * p.ldo + n, v);
-  };
   if (p.split == 1) {
     if (epi && !fail) {
+      with_type(p.out, p.out_dtype, [&](auto* out) {
+        auto* o = out + static_cast<int64_t>(m0) * p.ldo + n;
 #pragma unroll 1
-      for (int c = 0; c < kNT && c < tokens; c += 16) {
-        uint32_t x[16], y[16];
-        tmem_ld_32x32b_x16(taddr + c, x);
-        if (kGated) tmem_ld_32x32b_x16(taddr + kNT + c, y);
-        tmem_ld_wait();
+        for (int c = part * (kNT / 2); c < (part + 1) * (kNT / 2) && c < tokens; c += 8) {
+          uint32_t x[8], y[8];
+          tmem_ld_32x32b_x8(taddr + c, x);
+          if (kGated) tmem_ld_32x32b_x8(taddr + kNT + c, y);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c + i < tokens)
-            emit(c + i, acc_value<kE4M3>(x[i]), kGated ? acc_value<kE4M3>(y[i]) : 0.0f);
-      }
+          for (int i = 0; i < 8; ++i)
+            if (inside && c + i < tokens)
+              put(o + (c + i) * p.ldo,
+                  finish(c + i, acc_value<kE4M3>(x[i]), kGated ? acc_value<kE4M3>(y[i]) : 0.0f));
+        }
+      });
     }
   } else if constexpr (C::kSplits) {
-    // Every CTA's sums into its own ring (drained: all its MMAs are done), then
-    // CTA r of the cluster adds up tokens r, r + split, .. over the ranks in
-    // order and stores them.
-    fail = __syncthreads_or(fail) != 0;
-    uint32_t* red = reinterpret_cast<uint32_t*>(smem);
+    // Rank r of the cluster owns tokens [r * per, (r + 1) * per): every CTA
+    // stores its sums of them into r's memory, then r adds the ranks' sums in
+    // order. One cluster barrier in between (and one before, where the memory
+    // is the ring: its owner's MMAs are then done).
+    const int per = (tokens + p.split - 1) / p.split;
+    if (!C::kOwnRed) {
+      __syncwarp();
+      cluster_sync();
+    }
+    const uint32_t red = smem_u32(smem + C::kRedOff);
     if (epi && !fail) {
 #pragma unroll 1
-      for (int c = 0; c < C::kCols; c += 16) {
-        if (c % kNT >= tokens) continue;
-        uint32_t x[16];
-        tmem_ld_32x32b_x16(taddr + c, x);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) red[(c + i) * 128 + nl] = x[i];
-      }
-    }
-    cluster_sync();
-    if (epi && !fail) {
-      const uint32_t red_addr = smem_u32(red);
-      for (int m = ks; m < tokens; m += p.split) {
-        float sum[C::kW];
+      for (int c = part * (kNT / 2); c < (part + 1) * (kNT / 2) && c < tokens; c += 8) {
 #pragma unroll
         for (int w = 0; w < C::kW; ++w) {
-          uint32_t x[kMaxSplit];
+          uint32_t x[8];
+          tmem_ld_32x32b_x8(taddr + w * kNT + c, x);
+          tmem_ld_wait();
+          int owner = c / per, at = c - owner * per;
 #pragma unroll
-          for (int j = 0; j < kMaxSplit; ++j)
-            if (j < p.split)
-              x[j] = __float_as_uint(ld_cluster_f32(cluster_map(
-                  red_addr + ((w * kNT + m) * 128 + nl) * 4, static_cast<uint32_t>(j))));
-          if constexpr (kE4M3) {
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kMaxSplit; ++j)
-              if (j < p.split) s += __uint_as_float(x[j]);
-            sum[w] = s;
-          } else {
-            uint32_t s = 0;
-#pragma unroll
-            for (int j = 0; j < kMaxSplit; ++j)
-              if (j < p.split) s += x[j];
-            sum[w] = static_cast<float>(static_cast<int>(s));
+          for (int i = 0; i < 8; ++i) {
+            if (c + i < tokens) {
+              // [token of the owner][weight][source rank][channel]
+              const uint32_t to = red + ((at * C::kW + w) * p.split + ks) * 512 + nl * 4;
+              st_cluster_u32(cluster_map(to, owner), x[i]);
+              if (++at == per) {
+                at = 0;
+                ++owner;
+              }
+            }
           }
         }
-        emit(m, sum[0], sum[C::kW - 1]);
       }
     }
-    cluster_sync();  // no CTA leaves while another may read its sums
+    __syncwarp();
+    cluster_sync();
+    if (epi && !fail) {
+      const int first = ks * per;
+      auto total = [&](int m, int w) {
+        const uint32_t at = red + (((m - first) * C::kW + w) * p.split) * 512 + ch * 4;
+        if constexpr (kE4M3) {
+          float v = lds_f32(at);
+          for (int j = 1; j < p.split; ++j) v += lds_f32(at + j * 512);
+          return v;
+        } else {
+          uint32_t v = lds_u32(at);
+          for (int j = 1; j < p.split; ++j) v += lds_u32(at + j * 512);
+          return static_cast<float>(static_cast<int>(v));
+        }
+      };
+      with_type(p.out, p.out_dtype, [&](auto* out) {
+        auto* o = out + static_cast<int64_t>(m0) * p.ldo + n;
+#pragma unroll 4
+        for (int m = first + (et >> 7); m < min(first + per, tokens); m += 2) {
+          const float x = total(m, 0);
+          const float v = finish(m, x, kGated ? total(m, C::kW - 1) : 0.0f);
+          if (inside) put(o + m * p.ldo, v);
+        }
+      });
+    }
   }
 
   if (fail && warp == kTmaWarp && lane == 0) {
@@ -374,7 +421,9 @@ struct PairCfg {
   static constexpr int kStages = 6;
   static constexpr int kBarOff = kStages * kStageBytes;
   static constexpr int kScaleOff = kBarOff + 256;           // [2][256] scales, [2][256] bias
-  static constexpr int kSmem = kScaleOff + 4 * 256 * 4 + 1024;
+  static constexpr int kTurnOff = kScaleOff + 4 * 256 * 4;  // per epilogue warp [32][17] floats
+  static constexpr int kTurnBytes = 32 * 17 * 4;
+  static constexpr int kSmem = kTurnOff + kEpiWarps * kTurnBytes + 1024;
   static constexpr int kAccCols = 256;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -399,7 +448,7 @@ __device__ __forceinline__ void pair_unit(int u, const Params& p, int& tm, int& 
 }
 
 template <bool kE4M3, bool kGated>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     w8a8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmW0,
                      const __grid_constant__ CUtensorMap tmW1, const Params p) {
@@ -429,7 +478,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 2 * kPairEpiWarps);
+      mbar_init(&acc_empty[i], 2 * kEpiWarps);
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
@@ -516,7 +565,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // this unit's channel scales (gate then up) and bias
       float* sc = s_scale + ab * 256;
       float* bs = s_bias + ab * 256;
-      for (int i = et; i < (kGated ? 2 * outs : outs); i += kPairEpiWarps * 32) {
+      for (int i = et; i < (kGated ? 2 * outs : outs); i += kEpiThreads) {
         const int w = kGated && i >= outs ? 1 : 0;
         const int n = n0 + i - w * outs;
         sc[i] = n < p.N ? p.w_scale[w][n] : 0.0f;
@@ -527,7 +576,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // one barrier a unit: the scales are in place, and the warps agree on
       // whether the wait ran out (none is left waiting for one that gave up)
       fail = named_bar_or(
-          1, kPairEpiWarps * 32,
+          1, kEpiThreads,
           !mbar_wait(&acc_full[ab], (local >> 1) & 1, p.status, kSiteW8PairEpilogue));
       if (fail) break;
       tc_fence_after();
@@ -538,21 +587,44 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         tmem_ld_32x32b_x32(taddr + c, x);
         if (kGated) tmem_ld_32x32b_x32(taddr + outs + c, y);
         tmem_ld_wait();
-        if (row < p.M) {
+        auto value = [&](int i) {
+          const float v = acc_value<kE4M3>(x[i]) * sa * sc[c + i];
+          if constexpr (kGated)
+            return gated(v, acc_value<kE4M3>(y[i]) * sa * sc[outs + c + i], p.act);
+          return p.bias != nullptr ? v + bs[c + i] : v;
+        };
+        if (p.rows16) {
+          if (row < p.M) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float v[8];
+            for (int i = 0; i < 32; i += 8) {
+              float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              v[e] = acc_value<kE4M3>(x[i + e]) * sa * sc[c + i + e];
-              if constexpr (kGated)
-                v[e] = gated(v[e], acc_value<kE4M3>(y[i + e]) * sa * sc[outs + c + i + e], p.act);
-              else if (p.bias != nullptr)
-                v[e] += bs[c + i + e];
+              for (int e = 0; e < 8; ++e) v[e] = value(i + e);
+              const int n = n0 + c + i;
+              if (n < p.N)
+                store_eight(p.out, p.out_dtype, static_cast<int64_t>(row) * p.ldo + n, v, p.N - n);
             }
-            const int n = n0 + c + i;
-            if (n < p.N)
-              store_eight(p.out, p.out_dtype, static_cast<int64_t>(row) * p.ldo + n, v, p.N - n);
+          }
+        } else {
+          // Rows off 16-byte boundaries: sixteen columns at a time through
+          // shared memory, so that a warp stores two rows' runs at once (single
+          // stores of 32 rows took 52 us for 333 x 1111 x 1001, DIRECT).
+          float* turn = reinterpret_cast<float*>(smem + C::kTurnOff) + (warp - kEpiWarp0) * (32 * 17);
+          const int64_t row0 = static_cast<int64_t>(row) - lane;
+#pragma unroll
+          for (int g = 0; g < 32; g += 16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) turn[lane * 17 + i] = value(g + i);
+            __syncwarp();
+            const int n = n0 + c + g + (lane & 15);
+            with_type(p.out, p.out_dtype, [&](auto* out) {
+#pragma unroll
+              for (int r = 0; r < 32; r += 2) {
+                const int64_t at = row0 + r + (lane >> 4);
+                if (n < p.N && at < p.M) put(out + at * p.ldo + n, turn[(r + (lane >> 4)) * 17 + (lane & 15)]);
+              }
+            });
+            __syncwarp();
           }
         }
       }
@@ -591,6 +663,8 @@ Params params_of(const W8A8Args& g) {
   p.K = static_cast<int>(g.K);
   p.out_dtype = g.out_dtype;
   p.act = g.act;
+  p.rows16 = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 &&
+             (g.ldo * (g.out_dtype == PK_F32 ? 4 : 2)) % 16 == 0;
   p.split = 1;
   p.status = g.status;
   return p;
@@ -633,6 +707,7 @@ cudaError_t launch_swap(const W8A8Args& g, int split, cudaStream_t s, const char
   Params p = params_of(g);
   p.num_m = static_cast<int>(ceil_div(g.M, kNT));
   p.num_n = static_cast<int>(ceil_div(g.N, 128));
+  while ((split & (split - 1)) != 0) split &= split - 1;  // a divisor of kNT
   p.split = C::kSplits ? split : 1;
   const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;
   if (grid >= (1ll << 31)) return cudaErrorInvalidConfiguration;
@@ -673,7 +748,7 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
   if (tiles > slots && tail > 0 && 2 * tail <= slots) p.whole = tiles - tail;
   const int units = p.whole + 2 * (tiles - p.whole);
   return launch(w8a8_pair_kernel<kE4M3, kGated>, 2 * (units < slots ? units : slots),
-                kPairThreads, 2, PairCfg::kSmem, s, tm, p);
+                kThreads, 2, PairCfg::kSmem, s, tm, p);
 }
 
 // Which kernel, how many tokens a tile, how many K splits: from the sizes alone.
