@@ -9,7 +9,7 @@
 //
 // Two kernels:
 //  * w8a8_swap_kernel, few tokens: the weights are the MMA's 128-row operand,
-//    the tokens its 16..256 columns, one tile per CTA. The product is a weight
+//    the tokens its 16..256 columns (just as many as needed), one tile per CTA. The product is a weight
 //    stream there; K is split over a thread-block cluster when there are too
 //    few column tiles to keep every SM loading, and the partial sums meet in
 //    distributed shared memory (in rank order; no workspace, no atomics).
@@ -18,6 +18,8 @@
 //    next one's main loop. Gated: CTA 0 stages 128 gate channels and CTA 1 the
 //    same 128 up channels, so one MMA makes both halves and a row's epilogue
 //    thread holds gate and up of each of its 128 outputs.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "pk_common.cuh"
@@ -41,7 +43,9 @@ struct Params {
   int M, N, K;
   int out_dtype, act;
   int rows16;        // the output's rows start on 16-byte boundaries
-  int split;         // swap: CTAs per tile along K (the cluster)
+  // swap: CTAs per tile along K (the cluster), tokens of a tile (a multiple of
+  // 16), the ring, TMEM columns, whether the sums of a split have their own memory
+  int split, nt, stages, stage_bytes, tmem_cols, own_red;
   int num_m, num_n;  // tiles
   int whole;         // pair: units that are whole tiles; each later tile is two half-width units
   int* status;
@@ -51,6 +55,20 @@ struct Params {
 constexpr uint32_t idesc8(bool e4m3, int m, int n) {
   return (e4m3 ? 1u << 4 : (2u << 4) | (1u << 7) | (1u << 10)) |
          (static_cast<uint32_t>(n) >> 3 << 17) | (static_cast<uint32_t>(m) >> 4 << 24);
+}
+
+// One lane of a converged warp. The MMA warps run their loops with all lanes and
+// issue under this predicate: in a loop of one lane every operand of a
+// tcgen05.mma went from a vector to a uniform register, and a K tile's four MMAs
+// took ~550 cycles to issue, whatever their size.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 
 template <bool kE4M3>
@@ -132,96 +150,65 @@ __device__ __forceinline__ void with_type(void* out, int dtype, F f) {
   else f(static_cast<__half*>(out));
 }
 
+__device__ __forceinline__ void lds_floats(uint32_t addr, float (&v)[4]) {
+  const uint4 u = lds_v4(addr);
+  v[0] = __uint_as_float(u.x);
+  v[1] = __uint_as_float(u.y);
+  v[2] = __uint_as_float(u.z);
+  v[3] = __uint_as_float(u.w);
+}
+
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// Eight neighbouring outputs from a 16-byte boundary on, `valid` of them inside
-// the matrix.
-__device__ __forceinline__ void store_eight(void* out, int dtype, int64_t i, const float (&v)[8],
-                                            int valid) {
-  if (dtype == PK_F32) {
-    float* o = static_cast<float*>(out) + i;
-    if (valid >= 8) {
-      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      return;
-    }
-  } else {
-    uint16_t* o = static_cast<uint16_t*>(out) + i;
-    if (valid >= 8) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (dtype == PK_BF16) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&p);
-        } else {
-          const __half2 p = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&p);
-        }
-      }
-      *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
-      return;
-    }
+// Two outputs as one word of a 16-bit type.
+__device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {
+  if (dtype == PK_BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < valid) store_one(out, dtype, i + j, v[j]);
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens: D[channel, token], one 128-channel x kNT-token tile per CTA.
+// Few tokens: D[channel, token], one tile of 128 channels x nt tokens per CTA.
 // ---------------------------------------------------------------------------
-template <int kNT, bool kGated>
-struct SwapCfg {
-  static constexpr int kW = kGated ? 2 : 1;                 // weight tiles per stage
-  static constexpr int kWTile = 128 * kBK;                  // 16 KB
-  static constexpr int kStageBytes = kW * kWTile + kNT * kBK;
-  // up to 64 tokens two CTAs share an SM when one weight is streamed
-  static constexpr int kBudget = !kGated && kNT <= 64 ? 110 * 1024 : 216 * 1024;
-  static constexpr int kCols = kW * kNT;                    // accumulator columns
-  static constexpr int kTmem = kCols < 32 ? 32 : kCols;
-  // partial sums of a K split: their own memory when small, else the drained ring
-  static constexpr int kRedBytes = kCols * 128 * 4;
-  static constexpr bool kOwnRed = kRedBytes <= 16 * 1024;
-  static constexpr int kStages = (kBudget - (kOwnRed ? kRedBytes : 0)) / kStageBytes;
-  static constexpr int kBarOff = kStages * kStageBytes;
-  static constexpr int kScaleOff = kBarOff + 256;
-  static constexpr int kRedOff = kOwnRed ? kScaleOff + kNT * 4 : 0;
-  static constexpr int kSmem = kScaleOff + kNT * 4 + (kOwnRed ? kRedBytes : 0) + 1024;
-  static constexpr bool kSplits = kOwnRed || kRedBytes <= kBarOff;
-  static_assert(kSmem <= 227 * 1024 && kTmem <= 512, "one CTA fits an SM");
-};
+constexpr int kWTile = 128 * kBK;  // 16 KB: one stage of 128 channels
+constexpr int kMaxTokens = 256;    // tokens of a tile: the MMA's columns
 
 constexpr int kMaxSplit = 8;
+constexpr int kSwapBars = 256;      // bytes for its barriers (at most 15 stages)
 
-template <bool kE4M3, int kNT, bool kGated>
+template <bool kE4M3, bool kGated>
 __global__ void __launch_bounds__(kThreads)
     w8a8_swap_kernel(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmW0,
                      const __grid_constant__ CUtensorMap tmW1, const Params p) {
-  using C = SwapCfg<kNT, kGated>;
-  constexpr int kStages = C::kStages;
+  constexpr int kW = kGated ? 2 : 1;  // weight tiles per stage
+  const int nt = p.nt, stages = p.stages, stage_bytes = p.stage_bytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* empty = full + kStages;
-  uint64_t* done = empty + kStages;
+  // after the ring: token scales, barriers, and (own_red) the sums of a K split
+  float* s_sa = reinterpret_cast<float*>(smem + stages * stage_bytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_sa + kMaxTokens);
+  uint64_t* empty = full + stages;
+  uint64_t* done = empty + stages;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // split fastest (the cluster), then the token tiles that share a weight tile
   const int ks = static_cast<int>(blockIdx.x % p.split);
   const int tile = static_cast<int>(blockIdx.x / p.split);
-  const int m0 = (tile % p.num_m) * kNT, n0 = (tile / p.num_m) * 128;
+  const int m0 = (tile % p.num_m) * nt, n0 = (tile / p.num_m) * 128;
   const int k_tiles = (p.K + kBK - 1) / kBK;
   const int kt0 = static_cast<int>(static_cast<int64_t>(ks) * k_tiles / p.split);
   const int kt1 = static_cast<int>(static_cast<int64_t>(ks + 1) * k_tiles / p.split);
 
   if (warp == kTmaWarp && lane == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -232,69 +219,84 @@ __global__ void __launch_bounds__(kThreads)
     if (kGated) tma_prefetch_desc(&tmW1);
     // the first weights start towards L2 while the previous kernel ends (a
     // hint: nothing is read that it may still write)
-    for (int kt = kt0; kt < kt1 && kt < kt0 + kStages; ++kt) {
+    for (int kt = kt0; kt < kt1 && kt < kt0 + stages; ++kt) {
       tma_prefetch_l2_2d(&tmW0, kt * kBK, n0);
       if (kGated) tma_prefetch_l2_2d(&tmW1, kt * kBK, n0);
     }
   }
-  if (warp == kMmaWarp) tmem_alloc(tmem_holder, C::kTmem);
+  if (warp == kMmaWarp) tmem_alloc(tmem_holder, p.tmem_cols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   // a CTA's own memory for sums takes them from a CTA that has started
-  if (C::kOwnRed && p.split > 1) cluster_sync();
+  if (p.own_red && p.split > 1) cluster_sync();
   griddep_wait();
   griddep_launch_dependents();
 
   bool fail = false;
   int issued = 0;
   if (warp == kTmaWarp) {
-    if (lane == 0) {
-      for (int kt = kt0, it = 0; kt < kt1; ++kt, ++it) {
-        const int st = it % kStages;
-        if (it >= kStages)
-          fail = !mbar_wait(&empty[st], ((it / kStages) - 1) & 1, p.status, kSiteW8SwapProducer);
-        if (fail) break;
-        uint8_t* base = smem + st * C::kStageBytes;
-        mbar_arrive_expect_tx(&full[st], C::kStageBytes);
-        tma_load_2d(base, &tmW0, &full[st], kt * kBK, n0);
-        if (kGated) tma_load_2d(base + C::kWTile, &tmW1, &full[st], kt * kBK, n0);
-        tma_load_2d(base + C::kW * C::kWTile, &tmA, &full[st], kt * kBK, m0);
-        issued = it + 1;
+    uint8_t* base = smem;
+    uint64_t* bar = full;
+    uint32_t parity = 1;  // a fresh barrier's previous phase: the first round does not wait
+    for (int kt = kt0; kt < kt1; ++kt) {
+      fail = __any_sync(0xffffffffu, !mbar_wait(bar + stages, parity, p.status, kSiteW8SwapProducer));
+      if (fail) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar, stage_bytes);
+        tma_load_2d(base, &tmW0, bar, kt * kBK, n0);
+        if (kGated) tma_load_2d(base + kWTile, &tmW1, bar, kt * kBK, n0);
+        tma_load_2d(base + kW * kWTile, &tmA, bar, kt * kBK, m0);
+      }
+      __syncwarp();
+      ++issued;
+      base += stage_bytes;
+      if (++bar == empty) {
+        bar = full;
+        base = smem;
+        parity ^= 1;
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t kIdesc = idesc8(kE4M3, 128, kNT);
-      for (int kt = kt0, it = 0; kt < kt1; ++kt, ++it) {
-        const int st = it % kStages;
-        fail = !mbar_wait(&full[st], (it / kStages) & 1, p.status, kSiteW8SwapMma);
-        if (fail) break;
-        tc_fence_after();
-        const uint32_t w_base = smem_u32(smem + st * C::kStageBytes);
-        const uint32_t a_base = w_base + C::kW * C::kWTile;
+    const uint32_t idesc = idesc8(kE4M3, 128, nt);
+    const uint64_t desc0 = make_smem_desc(0, 16, 1024);  // a tile at address 0
+    uint32_t w_base = smem_u32(smem), acc = 0, parity = 0;
+    uint64_t* bar = full;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      // a warp gives up as one
+      fail = __any_sync(0xffffffffu, !mbar_wait(bar, parity, p.status, kSiteW8SwapMma));
+      if (fail) break;
+      if (elect_one()) {
+        const uint64_t wd = desc0 + (w_base >> 4), ad = wd + (kW * kWTile >> 4);
 #pragma unroll
         for (int s = 0; s < kKSteps; ++s) {
-          const uint64_t ad = make_smem_desc(a_base + s * 32, 16, 1024);
 #pragma unroll
-          for (int w = 0; w < C::kW; ++w)
-            umma8<kE4M3>(tmem + w * kNT, make_smem_desc(w_base + w * C::kWTile + s * 32, 16, 1024),
-                         ad, kIdesc, (it > 0 || s > 0) ? 1u : 0u);
+          for (int w = 0; w < kW; ++w)
+            umma8<kE4M3>(tmem + w * nt, wd + ((w * kWTile + s * 32) >> 4), ad + (s * 32 >> 4),
+                         idesc, s > 0 ? 1u : acc);
         }
-        umma_commit(&empty[st]);
+        umma_commit(bar + stages);
+        if (kt + 1 == kt1) umma_commit(done);
       }
-      if (!fail) umma_commit(done);
+      __syncwarp();
+      acc = 1;
+      w_base += stage_bytes;
+      if (++bar == empty) {
+        bar = full;
+        w_base = smem_u32(smem);
+        parity ^= 1;
+      }
     }
   }
 
   // ---- epilogue: a thread holds one channel, the columns are tokens ----
   const int q = warp & 3;  // TMEM lane quarter this warp may access
   const int nl = q * 32 + lane;
-  const int tokens = min(kNT, p.M - m0);
+  const int tokens = min(nt, p.M - m0);
   const bool epi = warp >= kEpiWarp0;
   const int part = (warp - kEpiWarp0) >> 2;  // which half of the tokens (epilogue warps)
-  float* s_sa = reinterpret_cast<float*>(smem + C::kScaleOff);
+  const uint32_t sa_addr = smem_u32(s_sa);
   const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
   // this thread's channel and what its epilogue multiplies and adds
   const int et = tid - kEpiWarp0 * 32;
@@ -302,16 +304,15 @@ __global__ void __launch_bounds__(kThreads)
   const int n = n0 + ch;
   const bool inside = epi && n < p.N;
   const bool biased = !kGated && p.bias != nullptr;
-  float sw[C::kW], bias = 0.0f;
-  auto finish = [&](int m, float x, float y) {
-    const float sa = s_sa[m];
+  float sw[kW], bias = 0.0f;
+  auto finish = [&](float sa, float x, float y) {
     x = x * sa * sw[0];
-    if constexpr (kGated) return gated(x, y * sa * sw[C::kW - 1], p.act);
+    if constexpr (kGated) return gated(x, y * sa * sw[kW - 1], p.act);
     return biased ? x + bias : x;
   };
   if (epi) {
 #pragma unroll
-    for (int w = 0; w < C::kW; ++w) sw[w] = inside ? p.w_scale[w][n] : 0.0f;
+    for (int w = 0; w < kW; ++w) sw[w] = inside ? p.w_scale[w][n] : 0.0f;
     if (biased && inside) bias = p.bias[n];
     for (int m = et; m < tokens; m += kEpiThreads) s_sa[m] = p.a_scale[m0 + m];
     named_bar_sync(1, kEpiThreads);
@@ -322,46 +323,54 @@ __global__ void __launch_bounds__(kThreads)
   if (p.split == 1) {
     if (epi && !fail) {
       with_type(p.out, p.out_dtype, [&](auto* out) {
-        auto* o = out + static_cast<int64_t>(m0) * p.ldo + n;
+        // Eight tokens at a time: everything is read and computed before the
+        // first store, which the compiler must otherwise keep the next token's
+        // scale behind (110 cycles an output: 256 tokens took 7 us).
 #pragma unroll 1
-        for (int c = part * (kNT / 2); c < (part + 1) * (kNT / 2) && c < tokens; c += 8) {
+        for (int c = part * (nt / 2); c < (part + 1) * (nt / 2) && c < tokens; c += 8) {
           uint32_t x[8], y[8];
           tmem_ld_32x32b_x8(taddr + c, x);
-          if (kGated) tmem_ld_32x32b_x8(taddr + kNT + c, y);
+          if (kGated) tmem_ld_32x32b_x8(taddr + nt + c, y);
+          const uint4 s0 = lds_v4(sa_addr + c * 4), s1 = lds_v4(sa_addr + c * 4 + 16);
+          const uint32_t sa[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
           tmem_ld_wait();
+          float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (inside && c + i < tokens)
-              put(o + (c + i) * p.ldo,
-                  finish(c + i, acc_value<kE4M3>(x[i]), kGated ? acc_value<kE4M3>(y[i]) : 0.0f));
+            v[i] = finish(__uint_as_float(sa[i]), acc_value<kE4M3>(x[i]),
+                          kGated ? acc_value<kE4M3>(y[i]) : 0.0f);
+          auto* o = out + static_cast<int64_t>(m0 + c) * p.ldo + n;
+#pragma unroll
+          for (int i = 0; i < 8; ++i, o += p.ldo)
+            if (inside && c + i < tokens) put(o, v[i]);
         }
       });
     }
-  } else if constexpr (C::kSplits) {
+  } else {
     // Rank r of the cluster owns tokens [r * per, (r + 1) * per): every CTA
     // stores its sums of them into r's memory, then r adds the ranks' sums in
     // order. One cluster barrier in between (and one before, where the memory
     // is the ring: its owner's MMAs are then done).
     const int per = (tokens + p.split - 1) / p.split;
-    if (!C::kOwnRed) {
+    if (!p.own_red) {
       __syncwarp();
       cluster_sync();
     }
-    const uint32_t red = smem_u32(smem + C::kRedOff);
+    const uint32_t red = smem_u32(p.own_red ? smem + stages * stage_bytes + kMaxTokens * 4 + kSwapBars : smem);
     if (epi && !fail) {
 #pragma unroll 1
-      for (int c = part * (kNT / 2); c < (part + 1) * (kNT / 2) && c < tokens; c += 8) {
+      for (int c = part * (nt / 2); c < (part + 1) * (nt / 2) && c < tokens; c += 8) {
 #pragma unroll
-        for (int w = 0; w < C::kW; ++w) {
+        for (int w = 0; w < kW; ++w) {
           uint32_t x[8];
-          tmem_ld_32x32b_x8(taddr + w * kNT + c, x);
+          tmem_ld_32x32b_x8(taddr + w * nt + c, x);
           tmem_ld_wait();
           int owner = c / per, at = c - owner * per;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (c + i < tokens) {
               // [token of the owner][weight][source rank][channel]
-              const uint32_t to = red + ((at * C::kW + w) * p.split + ks) * 512 + nl * 4;
+              const uint32_t to = red + ((at * kW + w) * p.split + ks) * 512 + nl * 4;
               st_cluster_u32(cluster_map(to, owner), x[i]);
               if (++at == per) {
                 at = 0;
@@ -377,24 +386,37 @@ __global__ void __launch_bounds__(kThreads)
     if (epi && !fail) {
       const int first = ks * per;
       auto total = [&](int m, int w) {
-        const uint32_t at = red + (((m - first) * C::kW + w) * p.split) * 512 + ch * 4;
+        const uint32_t at = red + (((m - first) * kW + w) * p.split) * 512 + ch * 4;
         if constexpr (kE4M3) {
           float v = lds_f32(at);
-          for (int j = 1; j < p.split; ++j) v += lds_f32(at + j * 512);
+#pragma unroll
+          for (int j = 1; j < kMaxSplit; ++j)
+            if (j < p.split) v += lds_f32(at + j * 512);
           return v;
         } else {
           uint32_t v = lds_u32(at);
-          for (int j = 1; j < p.split; ++j) v += lds_u32(at + j * 512);
+#pragma unroll
+          for (int j = 1; j < kMaxSplit; ++j)
+            if (j < p.split) v += lds_u32(at + j * 512);
           return static_cast<float>(static_cast<int>(v));
         }
       };
       with_type(p.out, p.out_dtype, [&](auto* out) {
-        auto* o = out + static_cast<int64_t>(m0) * p.ldo + n;
-#pragma unroll 4
-        for (int m = first + (et >> 7); m < min(first + per, tokens); m += 2) {
-          const float x = total(m, 0);
-          const float v = finish(m, x, kGated ? total(m, C::kW - 1) : 0.0f);
-          if (inside) put(o + m * p.ldo, v);
+        const int last = min(first + per, tokens);
+        // four tokens (of this thread's parity) at a time, read before stored
+#pragma unroll 1
+        for (int m = first + (et >> 7); m < last; m += 8) {
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int mm = min(m + 2 * i, last - 1);
+            v[i] = finish(lds_f32(sa_addr + mm * 4), total(mm, 0),
+                          kGated ? total(mm, kW - 1) : 0.0f);
+          }
+          auto* o = out + static_cast<int64_t>(m0 + m) * p.ldo + n;
+#pragma unroll
+          for (int i = 0; i < 4; ++i, o += 2 * p.ldo)
+            if (inside && m + 2 * i < last) put(o, v[i]);
         }
       });
     }
@@ -402,11 +424,11 @@ __global__ void __launch_bounds__(kThreads)
 
   if (fail && warp == kTmaWarp && lane == 0) {
     // copies already issued land before the CTA's shared memory is released
-    for (int s = 0; s < issued; ++s) mbar_wait(&full[s % kStages], (s / kStages) & 1, nullptr, 0);
+    for (int s = 0; s < issued; ++s) mbar_wait(&full[s % stages], (s / stages) & 1, nullptr, 0);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmem);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, p.tmem_cols);
 }
 
 // ---------------------------------------------------------------------------
@@ -491,27 +513,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   griddep_wait();
+  griddep_launch_dependents();
 
   bool fail = false;
   if (warp == kTmaWarp) {
-    if (lane == 0) {
-      const CUtensorMap* tmW = kGated && rank == 1 ? &tmW1 : &tmW0;
-      const uint32_t full0 = cluster_map(smem_u32(&full[0]), 0);
-      int it = 0;
-      for (int u = pair; u < num_units && !fail; u += npairs) {
-        int tm, tn, half;
-        pair_unit(u, p, tm, tn, half);
-        const int row = tm * 256 + rank * 128;
-        // whole: 128 channels in two boxes; half: 64 of the half's outputs
-        const int boxes = half < 0 ? 2 : 1;
-        const int col = tn * kTileN + (kGated ? (half < 0 ? 0 : half * 64)
-                                              : (half < 0 ? rank * 128 : half * 128 + rank * 64));
-        const uint32_t tx = 2u * (C::kATile + boxes * C::kBBox);
-        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
-          const int st = it % C::kStages;
-          if (it >= C::kStages)
-            fail = !mbar_wait(&empty[st], ((it / C::kStages) - 1) & 1, p.status, kSiteW8PairProducer);
-          if (fail) break;
+    const CUtensorMap* tmW = kGated && rank == 1 ? &tmW1 : &tmW0;
+    const uint32_t full0 = cluster_map(smem_u32(&full[0]), 0);
+    int st = 0;
+    uint32_t parity = 1;
+    for (int u = pair; u < num_units && !fail; u += npairs) {
+      int tm, tn, half;
+      pair_unit(u, p, tm, tn, half);
+      const int row = tm * 256 + rank * 128;
+      // whole: 128 channels in two boxes; half: 64 of the half's outputs
+      const int boxes = half < 0 ? 2 : 1;
+      const int col = tn * kTileN + (kGated ? (half < 0 ? 0 : half * 64)
+                                            : (half < 0 ? rank * 128 : half * 128 + rank * 64));
+      const uint32_t tx = 2u * (C::kATile + boxes * C::kBBox);
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        fail = __any_sync(0xffffffffu, !mbar_wait(&empty[st], parity, p.status, kSiteW8PairProducer));
+        if (fail) break;
+        if (elect_one()) {
           uint8_t* base = smem + st * C::kStageBytes;
           const uint32_t bar = full0 + st * 8;
           if (rank == 0) mbar_arrive_expect_tx(&full[st], tx);
@@ -519,34 +541,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int b = 0; b < boxes; ++b)
             tma_load_2d_pair(base + C::kATile + b * C::kBBox, tmW, bar, kt * kBK, col + b * 64);
         }
+        __syncwarp();
+        if (++st == C::kStages) {
+          st = 0;
+          parity ^= 1;
+        }
       }
     }
   } else if (warp == kMmaWarp) {
-    if (rank == 0 && lane == 0) {
-      int it = 0, local = 0;
+    if (rank == 0) {
+      const uint64_t desc0 = make_smem_desc(0, 16, 1024);
+      const uint32_t base0 = smem_u32(smem);
+      int local = 0, st = 0;
+      uint32_t parity = 0;
       for (int u = pair; u < num_units && !fail; u += npairs, ++local) {
         const uint32_t idesc = u < p.whole ? idesc8(kE4M3, 256, 256) : idesc8(kE4M3, 256, 128);
         const int ab = local & 1;
         if (local >= 2)
-          fail = !mbar_wait_cluster(&acc_empty[ab], ((local >> 1) - 1) & 1, p.status, kSiteW8PairMma);
+          fail = __any_sync(0xffffffffu, !mbar_wait_cluster(&acc_empty[ab], ((local >> 1) - 1) & 1,
+                                                            p.status, kSiteW8PairMma));
         if (fail) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem + ab * C::kAccCols;
-        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
-          const int st = it % C::kStages;
-          fail = !mbar_wait(&full[st], (it / C::kStages) & 1, p.status, kSiteW8PairMma);
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          fail = __any_sync(0xffffffffu, !mbar_wait(&full[st], parity, p.status, kSiteW8PairMma));
           if (fail) break;
-          tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + st * C::kStageBytes);
+          if (elect_one()) {
+            const uint64_t ad = desc0 + ((base0 + st * C::kStageBytes) >> 4);
+            const uint64_t bd = ad + (C::kATile >> 4);
 #pragma unroll
-          for (int s = 0; s < kKSteps; ++s)
-            umma8_pair<kE4M3>(d_tmem, make_smem_desc(a_base + s * 32, 16, 1024),
-                              make_smem_desc(a_base + C::kATile + s * 32, 16, 1024), idesc,
-                              (kt > 0 || s > 0) ? 1u : 0u);
-          umma_commit_pair(&empty[st]);
+            for (int s = 0; s < kKSteps; ++s)
+              umma8_pair<kE4M3>(d_tmem, ad + (s * 32 >> 4), bd + (s * 32 >> 4), idesc,
+                                (kt > 0 || s > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[st]);
+            if (kt + 1 == k_tiles) umma_commit_pair(&acc_full[ab]);
+          }
+          __syncwarp();
+          if (++st == C::kStages) {
+            st = 0;
+            parity ^= 1;
+          }
         }
-        if (fail) break;
-        umma_commit_pair(&acc_full[ab]);
       }
     }
   } else {
@@ -565,6 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // this unit's channel scales (gate then up) and bias
       float* sc = s_scale + ab * 256;
       float* bs = s_bias + ab * 256;
+      const uint32_t sc_addr = smem_u32(sc);
+      constexpr int kBiasOff = 2 * 256 * 4;  // from a unit's scales to its bias
       for (int i = et; i < (kGated ? 2 * outs : outs); i += kEpiThreads) {
         const int w = kGated && i >= outs ? 1 : 0;
         const int n = n0 + i - w * outs;
@@ -587,41 +624,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_x32(taddr + c, x);
         if (kGated) tmem_ld_32x32b_x32(taddr + outs + c, y);
         tmem_ld_wait();
-        auto value = [&](int i) {
-          const float v = acc_value<kE4M3>(x[i]) * sa * sc[c + i];
-          if constexpr (kGated)
-            return gated(v, acc_value<kE4M3>(y[i]) * sa * sc[outs + c + i], p.act);
-          return p.bias != nullptr ? v + bs[c + i] : v;
-        };
+        // all values before the first store: it would hold back later reads
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float w[4];
+          lds_floats(sc_addr + (c + i) * 4, w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i + e] = acc_value<kE4M3>(x[i + e]) * sa * w[e];
+          if constexpr (kGated) {
+            lds_floats(sc_addr + (outs + c + i) * 4, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[i + e] = gated(v[i + e], acc_value<kE4M3>(y[i + e]) * sa * w[e], p.act);
+          } else if (p.bias != nullptr) {
+            lds_floats(sc_addr + kBiasOff + (c + i) * 4, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i + e] += w[e];
+          }
+        }
+        const uint32_t turn = smem_u32(smem + C::kTurnOff) + (warp - kEpiWarp0) * C::kTurnBytes;
+        const int64_t row0 = static_cast<int64_t>(row) - lane;
         if (p.rows16) {
-          if (row < p.M) {
+          // 64 bytes of each of the warp's rows through shared memory (the
+          // 16-byte pieces of a row pair rotated so that neither side has bank
+          // conflicts), so that a store covers eight rows' whole sectors: stored
+          // by the row's own thread a tile's epilogue took 5 us.
+          const int elt = p.out_dtype == PK_F32 ? 4 : 2;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float v[8];
+          for (int g = 0; g < 2; ++g) {
+            if (g == 1 && elt == 2) break;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = value(i + e);
-              const int n = n0 + c + i;
-              if (n < p.N)
-                store_eight(p.out, p.out_dtype, static_cast<int64_t>(row) * p.ldo + n, v, p.N - n);
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t at = turn + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+              if (elt == 4)
+                sts_v4f(at, v[16 * g + 4 * j], v[16 * g + 4 * j + 1], v[16 * g + 4 * j + 2],
+                        v[16 * g + 4 * j + 3]);
+              else
+                sts_v4u(at, pack16(p.out_dtype, v[8 * j], v[8 * j + 1]),
+                        pack16(p.out_dtype, v[8 * j + 2], v[8 * j + 3]),
+                        pack16(p.out_dtype, v[8 * j + 4], v[8 * j + 5]),
+                        pack16(p.out_dtype, v[8 * j + 6], v[8 * j + 7]));
             }
+            __syncwarp();
+            const int j = lane & 3, per = 16 / elt;  // this lane's piece of a row, its outputs
+            const int n = n0 + c + 16 * g + j * per;
+#pragma unroll
+            for (int r = 0; r < 32; r += 8) {
+              const int rr = r + (lane >> 2);
+              const uint4 w = lds_v4(turn + rr * 64 + ((j ^ ((rr >> 1) & 3)) << 4));
+              if (n < p.N && row0 + rr < p.M) {
+                uint8_t* o = static_cast<uint8_t*>(p.out) + ((row0 + rr) * p.ldo + n) * elt;
+                if (n + per <= p.N) {
+                  *reinterpret_cast<uint4*>(o) = w;
+                } else {
+                  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    if (elt == 4) {
+                      if (n + k < p.N) reinterpret_cast<uint32_t*>(o)[k] = words[k];
+                    } else {
+                      if (n + 2 * k < p.N) reinterpret_cast<uint16_t*>(o)[2 * k] = static_cast<uint16_t>(words[k]);
+                      if (n + 2 * k + 1 < p.N) reinterpret_cast<uint16_t*>(o)[2 * k + 1] = static_cast<uint16_t>(words[k] >> 16);
+                    }
+                  }
+                }
+              }
+            }
+            __syncwarp();
           }
         } else {
           // Rows off 16-byte boundaries: sixteen columns at a time through
           // shared memory, so that a warp stores two rows' runs at once (single
           // stores of 32 rows took 52 us for 333 x 1111 x 1001, DIRECT).
-          float* turn = reinterpret_cast<float*>(smem + C::kTurnOff) + (warp - kEpiWarp0) * (32 * 17);
-          const int64_t row0 = static_cast<int64_t>(row) - lane;
 #pragma unroll
           for (int g = 0; g < 32; g += 16) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) turn[lane * 17 + i] = value(g + i);
+            for (int i = 0; i < 16; ++i) sts_f32(turn + (lane * 17 + i) * 4, v[g + i]);
             __syncwarp();
             const int n = n0 + c + g + (lane & 15);
             with_type(p.out, p.out_dtype, [&](auto* out) {
 #pragma unroll
               for (int r = 0; r < 32; r += 2) {
                 const int64_t at = row0 + r + (lane >> 4);
-                if (n < p.N && at < p.M) put(out + at * p.ldo + n, turn[(r + (lane >> 4)) * 17 + (lane & 15)]);
+                const float f = lds_f32(turn + ((r + (lane >> 4)) * 17 + (lane & 15)) * 4);
+                if (n < p.N && at < p.M) put(out + at * p.ldo + n, f);
               }
             });
             __syncwarp();
@@ -644,6 +731,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 bool rows_map(CUtensorMap* m, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows,
               const char** why) {
   return encode_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, K, rows, ld, kBK, box_rows,
@@ -692,39 +781,66 @@ cudaError_t launch(Kernel kernel, int grid, int threads, int cluster, int smem, 
   return cudaLaunchKernelEx(&cfg, kernel, tm[0], tm[1], tm[2], p);
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Which kernel, how many tokens a tile, how many K splits: from the sizes alone.
+struct Plan {
+  bool pair;
+  int nt, split;
+  bool deep;  // swap: the ring may take a whole SM's shared memory
+};
 
-template <bool kE4M3, int kNT, bool kGated>
-cudaError_t launch_swap(const W8A8Args& g, int split, cudaStream_t s, const char** why) {
-  using C = SwapCfg<kNT, kGated>;
+// Shared memory of a swap CTA: its ring, and what follows it.
+struct SwapSmem {
+  int stages, stage_bytes, own_red, bytes;
+  bool fits;
+};
+
+SwapSmem swap_smem(const Plan& plan, bool gated, int64_t k_tiles) {
+  SwapSmem c{};
+  const int w = gated ? 2 : 1;
+  const int sums = plan.split > 1 ? w * plan.nt * 128 * 4 : 0;
+  c.stage_bytes = w * kWTile + plan.nt * kBK;
+  c.own_red = sums > 0 && sums <= 16 * 1024;
+  const int rest = kMaxTokens * 4 + kSwapBars + (c.own_red ? sums : 0) + 1024;
+  // two CTAs an SM where half the memory holds four stages
+  const int half = 113 * 1024 - rest, whole = 226 * 1024 - rest;
+  c.stages = (!plan.deep && half / c.stage_bytes >= 4 ? half : whole) / c.stage_bytes;
+  c.stages = static_cast<int>(std::min<int64_t>(std::min(c.stages, 12), ceil_div(k_tiles, plan.split)));
+  // sums without memory of their own go into the drained ring
+  if (sums > 0 && !c.own_red)
+    while (c.stages * c.stage_bytes < sums && (c.stages + 1) * c.stage_bytes <= whole) ++c.stages;
+  c.fits = sums == 0 || c.own_red || sums <= c.stages * c.stage_bytes;
+  c.bytes = c.stages * c.stage_bytes + rest;
+  return c;
+}
+
+template <bool kE4M3, bool kGated>
+cudaError_t launch_swap(const W8A8Args& g, const Plan& plan, cudaStream_t s, const char** why) {
+  const SwapSmem c = swap_smem(plan, kGated, ceil_div(g.K, kBK));
+  if (!c.fits) {
+    *why = "the sums of the K split do not fit shared memory";
+    return cudaErrorInvalidValue;
+  }
   CUtensorMap tm[3];
-  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, kNT, why) ||
+  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, plan.nt, why) ||
       !rows_map(&tm[1], g.w[0], g.N, g.K, g.ldw[0], 128, why))
     return cudaErrorInvalidValue;
   tm[2] = tm[1];
   if (kGated && !rows_map(&tm[2], g.w[1], g.N, g.K, g.ldw[1], 128, why))
     return cudaErrorInvalidValue;
   Params p = params_of(g);
-  p.num_m = static_cast<int>(ceil_div(g.M, kNT));
+  p.nt = plan.nt;
+  p.split = plan.split;
+  p.stages = c.stages;
+  p.stage_bytes = c.stage_bytes;
+  p.own_red = c.own_red;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < plan.nt * (kGated ? 2 : 1)) p.tmem_cols *= 2;
+  p.num_m = static_cast<int>(ceil_div(g.M, plan.nt));
   p.num_n = static_cast<int>(ceil_div(g.N, 128));
-  while ((split & (split - 1)) != 0) split &= split - 1;  // a divisor of kNT
-  p.split = C::kSplits ? split : 1;
   const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;
   if (grid >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-  return launch(w8a8_swap_kernel<kE4M3, kNT, kGated>, static_cast<int>(grid), kThreads, p.split,
-                C::kSmem, s, tm, p);
-}
-
-template <bool kE4M3, bool kGated>
-cudaError_t launch_swap_any(const W8A8Args& g, int nt, int split, cudaStream_t s,
-                            const char** why) {
-  switch (nt) {
-    case 16: return launch_swap<kE4M3, 16, kGated>(g, split, s, why);
-    case 32: return launch_swap<kE4M3, 32, kGated>(g, split, s, why);
-    case 64: return launch_swap<kE4M3, 64, kGated>(g, split, s, why);
-    case 128: return launch_swap<kE4M3, 128, kGated>(g, split, s, why);
-    default: return launch_swap<kE4M3, 256, kGated>(g, split, s, why);
-  }
+  return launch(w8a8_swap_kernel<kE4M3, kGated>, static_cast<int>(grid), kThreads, p.split, c.bytes,
+                s, tm, p);
 }
 
 template <bool kE4M3, bool kGated>
@@ -751,37 +867,85 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
                 kThreads, 2, PairCfg::kSmem, s, tm, p);
 }
 
-// Which kernel, how many tokens a tile, how many K splits: from the sizes alone.
-struct Plan {
-  bool pair;
-  int nt, split;
-};
+// Estimated microseconds of a plan, from the kernels' measured parts (what
+// matters is the order of the plans):
+//  * an SM takes in ~115 GB/s of tiles, and no more than its rings hold per
+//    ~1.45 us of memory latency; HBM delivers ~6.3 TB/s of weights;
+//  * a grid runs in rounds of the CTAs that are resident at once: at one CTA an
+//    SM 148, of clusters of 4 132, of clusters of 8 120;
+//  * swap: 3 us of launch and first loads; per token of a tile 13 ns of epilogue
+//    (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
+//  * pair: 6 us around the main loop, 32 KB per CTA and K tile (a half unit 24).
+constexpr float kSmBytes = 115e3f, kHbmBytes = 6.3e6f, kLatency = 1.45f;  // per us; us
+
+float plan_us(const Plan& plan, const W8A8Args& g) {
+  const float sms = static_cast<float>(num_sms());
+  const float w = g.gated ? 2.0f : 1.0f;
+  const int64_t k_tiles = ceil_div(g.K, kBK);
+  if (plan.pair) {
+    const int64_t num_m = ceil_div(g.M, 256), tiles = num_m * ceil_div(g.N, g.gated ? 128 : 256);
+    const int64_t slots = num_sms() / 2, tail = tiles % slots;
+    const float kt = static_cast<float>(k_tiles), weights = 256.0f * kBK / static_cast<float>(num_m);
+    auto wave = [&](int64_t units, float bytes) {
+      return kt * std::max(static_cast<float>(units) * weights / kHbmBytes, bytes / kSmBytes);
+    };
+    float us = 6.0f + static_cast<float>(tiles / slots) * wave(slots, 32768.0f);
+    if (tail > 0) us += wave(tail, tiles > slots && 2 * tail <= slots ? 24576.0f : 32768.0f);
+    return us;
+  }
+  const SwapSmem c = swap_smem(plan, g.gated, k_tiles);
+  const int occ = c.bytes <= 113 * 1024 ? 2 : 1;
+  const int64_t num_m = ceil_div(g.M, plan.nt);
+  const int64_t ctas = num_m * ceil_div(g.N, 128) * plan.split;
+  const float part = plan.split == 8 ? 120.0f / 148 : plan.split == 4 ? 132.0f / 148 : 1.0f;
+  const int64_t one = std::max<int64_t>(1, static_cast<int64_t>(sms * part));  // CTAs at one an SM
+  const float kt = static_cast<float>(ceil_div(k_tiles, plan.split));
+  const float ring = static_cast<float>(c.stages * c.stage_bytes);
+  auto round = [&](int64_t n) {
+    const float per_sm = static_cast<float>(ceil_div(n, one));
+    const float in = std::min(kSmBytes, per_sm * ring / kLatency);
+    return kt * std::max(static_cast<float>(n) * w * kWTile / static_cast<float>(num_m) / kHbmBytes,
+                         per_sm * static_cast<float>(c.stage_bytes) / in);
+  };
+  const float nt = static_cast<float>(plan.nt), split = static_cast<float>(plan.split);
+  const float epilogue = plan.split == 1
+                             ? nt * (g.gated ? 0.023f : 0.013f)
+                             : 0.4f + w * nt * (0.030f + 0.020f / split);
+  const int64_t full = ctas / (one * occ), rest = ctas % (one * occ);
+  float us = 3.0f + static_cast<float>(full) * (round(one * occ) + epilogue);
+  if (rest > 0) us += round(rest) + epilogue;
+  return us;
+}
 
 Plan plan_of(const W8A8Args& g) {
-  const int sms = num_sms();
-  Plan plan{false, 16, 1};
-  const int64_t pair_tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? 128 : 256);
-  if (g.M > 128 && pair_tiles >= sms / 2) {
-    plan.pair = true;
-    return plan;
-  }
-  while (plan.nt < 256 && plan.nt < g.M) plan.nt *= 2;
-  if (plan.nt > 128 && ceil_div(g.N, 128) * ceil_div(g.M, 256) < sms) plan.nt = 128;
-  const int64_t tiles = ceil_div(g.N, 128) * ceil_div(g.M, plan.nt);
-  const int64_t slots = !g.gated && plan.nt <= 64 ? 2 * sms : sms;
-  int64_t split = slots / tiles;
   const int64_t k_tiles = ceil_div(g.K, kBK);
-  if (split > k_tiles) split = k_tiles;
-  if (split > kMaxSplit) split = kMaxSplit;
-  while (plan.split * 2 <= split) plan.split *= 2;
-  return plan;
+  Plan best{true, 0, 1, false};
+  float least = g.M > 128 ? plan_us(best, g) : 1e30f;
+  // token tiles as even as sixteens allow, from as few as there can be to 16 wide
+  for (int64_t num_m = ceil_div(g.M, kMaxTokens), nt = 0, last = 0; num_m <= 16; ++num_m) {
+    nt = ceil_div(ceil_div(g.M, num_m), 16) * 16;
+    if (nt == last) continue;
+    last = nt;
+    for (int split = 1; split <= kMaxSplit && split <= k_tiles; split *= 2) {
+      for (int deep = 0; deep < 2; ++deep) {
+        const Plan plan{false, static_cast<int>(nt), split, deep != 0};
+        if (!swap_smem(plan, g.gated, k_tiles).fits) continue;
+        const float us = plan_us(plan, g);
+        if (us < least) {
+          least = us;
+          best = plan;
+        }
+      }
+    }
+    if (nt == 16) break;
+  }
+  return best;
 }
 
 template <bool kE4M3, bool kGated>
 cudaError_t launch_typed(const W8A8Args& g, cudaStream_t s, const char** why) {
   const Plan plan = plan_of(g);
-  if (plan.pair) return launch_pair<kE4M3, kGated>(g, s, why);
-  return launch_swap_any<kE4M3, kGated>(g, plan.nt, plan.split, s, why);
+  return plan.pair ? launch_pair<kE4M3, kGated>(g, s, why) : launch_swap<kE4M3, kGated>(g, plan, s, why);
 }
 
 }  // namespace
