@@ -46,6 +46,7 @@ struct Params {
   // swap: CTAs per tile along K (the cluster), tokens of a tile (a multiple of
   // 16), the ring, TMEM columns, whether the sums of a split have their own memory
   int split, nt, stages, stage_bytes, tmem_cols, own_red;
+  int pieces;        // swap: accumulators that a CTA's K range is summed in
   int num_m, num_n;  // tiles
   int whole;         // pair: units that are whole tiles; each later tile is two half-width units
   int* status;
@@ -261,7 +262,9 @@ __global__ void __launch_bounds__(kThreads)
   } else if (warp == kMmaWarp) {
     const uint32_t idesc = idesc8(kE4M3, 128, nt);
     const uint64_t desc0 = make_smem_desc(0, 16, 1024);  // a tile at address 0
-    uint32_t w_base = smem_u32(smem), acc = 0, parity = 0;
+    uint32_t w_base = smem_u32(smem), parity = 0, d_tmem = tmem;
+    const int per_piece = (kt1 - kt0 + p.pieces - 1) / p.pieces;
+    int in_piece = 0;  // K tiles in the current accumulator
     uint64_t* bar = full;
     for (int kt = kt0; kt < kt1; ++kt) {
       // a warp gives up as one
@@ -273,14 +276,17 @@ __global__ void __launch_bounds__(kThreads)
         for (int s = 0; s < kKSteps; ++s) {
 #pragma unroll
           for (int w = 0; w < kW; ++w)
-            umma8<kE4M3>(tmem + w * nt, wd + ((w * kWTile + s * 32) >> 4), ad + (s * 32 >> 4),
-                         idesc, s > 0 ? 1u : acc);
+            umma8<kE4M3>(d_tmem + w * nt, wd + ((w * kWTile + s * 32) >> 4), ad + (s * 32 >> 4),
+                         idesc, s > 0 || in_piece > 0 ? 1u : 0u);
         }
         umma_commit(bar + stages);
         if (kt + 1 == kt1) umma_commit(done);
       }
       __syncwarp();
-      acc = 1;
+      if (++in_piece == per_piece) {
+        in_piece = 0;
+        d_tmem += kW * nt;
+      }
       w_base += stage_bytes;
       if (++bar == empty) {
         bar = full;
@@ -298,6 +304,23 @@ __global__ void __launch_bounds__(kThreads)
   const int part = (warp - kEpiWarp0) >> 2;  // which half of the tokens (epilogue warps)
   const uint32_t sa_addr = smem_u32(s_sa);
   const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  // eight accumulator columns, the pieces of K added up (used when the loads of
+  // a caller's tmem_ld_wait are in)
+  const int used = (kt1 - kt0 + p.pieces - 1) / p.pieces;
+  const int filled = (kt1 - kt0 + used - 1) / used;
+  auto load_sums = [&](int col, uint32_t (&x)[8]) {
+    tmem_ld_32x32b_x8(taddr + col, x);
+    if (kE4M3 && filled > 1) {
+      for (int i = 1; i < filled; ++i) {
+        uint32_t y[8];
+        tmem_ld_32x32b_x8(taddr + i * kW * nt + col, y);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(y[e]));
+      }
+    }
+  };
   // this thread's channel and what its epilogue multiplies and adds
   const int et = tid - kEpiWarp0 * 32;
   const int ch = p.split == 1 ? nl : et & 127;
@@ -329,8 +352,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll 1
         for (int c = part * (nt / 2); c < (part + 1) * (nt / 2) && c < tokens; c += 8) {
           uint32_t x[8], y[8];
-          tmem_ld_32x32b_x8(taddr + c, x);
-          if (kGated) tmem_ld_32x32b_x8(taddr + nt + c, y);
+          load_sums(c, x);
+          if (kGated) load_sums(nt + c, y);
           const uint4 s0 = lds_v4(sa_addr + c * 4), s1 = lds_v4(sa_addr + c * 4 + 16);
           const uint32_t sa[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
           tmem_ld_wait();
@@ -363,7 +386,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
           uint32_t x[8];
-          tmem_ld_32x32b_x8(taddr + w * nt + c, x);
+          load_sums(w * nt + c, x);
           tmem_ld_wait();
           int owner = c / per, at = c - owner * per;
 #pragma unroll
@@ -785,7 +808,8 @@ cudaError_t launch(Kernel kernel, int grid, int threads, int cluster, int smem, 
 struct Plan {
   bool pair;
   int nt, split;
-  bool deep;  // swap: the ring may take a whole SM's shared memory
+  bool deep;   // swap: the ring may take a whole SM's shared memory
+  int pieces;  // swap: accumulators of a CTA
 };
 
 // Shared memory of a swap CTA: its ring, and what follows it.
@@ -833,8 +857,9 @@ cudaError_t launch_swap(const W8A8Args& g, const Plan& plan, cudaStream_t s, con
   p.stages = c.stages;
   p.stage_bytes = c.stage_bytes;
   p.own_red = c.own_red;
+  p.pieces = plan.pieces;
   p.tmem_cols = 32;
-  while (p.tmem_cols < plan.nt * (kGated ? 2 : 1)) p.tmem_cols *= 2;
+  while (p.tmem_cols < plan.nt * (kGated ? 2 : 1) * plan.pieces) p.tmem_cols *= 2;
   p.num_m = static_cast<int>(ceil_div(g.M, plan.nt));
   p.num_n = static_cast<int>(ceil_div(g.N, 128));
   const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;
@@ -869,14 +894,18 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
 
 // Estimated microseconds of a plan, from the kernels' measured parts (what
 // matters is the order of the plans):
-//  * an SM takes in ~115 GB/s of tiles, and no more than its rings hold per
-//    ~1.45 us of memory latency; HBM delivers ~6.3 TB/s of weights;
+//  * an SM takes in ~150 GB/s of tiles, and no more than its rings hold per
+//    ~1.6 us of memory latency; HBM delivers ~6.3 TB/s of weights
+//    to all SMs, less to a part of them;
+//  * a CTA spends 0.1 us on a K tile's barriers and 30 ns on an MMA, or, from 114
+//    tokens on, the MMA's own nt / 2 cycles;
 //  * a grid runs in rounds of the CTAs that are resident at once: at one CTA an
 //    SM 148, of clusters of 4 132, of clusters of 8 120;
-//  * swap: 3 us of launch and first loads; per token of a tile 13 ns of epilogue
+//  * swap: 2.5 us of launch and first loads, 0.7 more where a CTA takes most of an
+//    SM's memory (the next kernel's CTAs then wait for it); per token of a tile 13 ns of epilogue
 //    (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
-//  * pair: 6 us around the main loop, 32 KB per CTA and K tile (a half unit 24).
-constexpr float kSmBytes = 115e3f, kHbmBytes = 6.3e6f, kLatency = 1.45f;  // per us; us
+//  * pair: 6 us around the main loop, 0.28 us a K tile (0.21 of a half unit).
+constexpr float kSmBytes = 150e3f, kHbmBytes = 6.3e6f, kLatency = 1.6f;  // per us; us
 
 float plan_us(const Plan& plan, const W8A8Args& g) {
   const float sms = static_cast<float>(num_sms());
@@ -886,11 +915,11 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
     const int64_t num_m = ceil_div(g.M, 256), tiles = num_m * ceil_div(g.N, g.gated ? 128 : 256);
     const int64_t slots = num_sms() / 2, tail = tiles % slots;
     const float kt = static_cast<float>(k_tiles), weights = 256.0f * kBK / static_cast<float>(num_m);
-    auto wave = [&](int64_t units, float bytes) {
-      return kt * std::max(static_cast<float>(units) * weights / kHbmBytes, bytes / kSmBytes);
+    auto wave = [&](int64_t units, float k_tile_us) {
+      return kt * std::max(static_cast<float>(units) * weights / kHbmBytes, k_tile_us);
     };
-    float us = 6.0f + static_cast<float>(tiles / slots) * wave(slots, 32768.0f);
-    if (tail > 0) us += wave(tail, tiles > slots && 2 * tail <= slots ? 24576.0f : 32768.0f);
+    float us = 6.0f + static_cast<float>(tiles / slots) * wave(slots, 0.28f);
+    if (tail > 0) us += wave(tail, tiles > slots && 2 * tail <= slots ? 0.21f : 0.28f);
     return us;
   }
   const SwapSmem c = swap_smem(plan, g.gated, k_tiles);
@@ -901,37 +930,59 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
   const int64_t one = std::max<int64_t>(1, static_cast<int64_t>(sms * part));  // CTAs at one an SM
   const float kt = static_cast<float>(ceil_div(k_tiles, plan.split));
   const float ring = static_cast<float>(c.stages * c.stage_bytes);
-  auto round = [&](int64_t n) {
-    const float per_sm = static_cast<float>(ceil_div(n, one));
-    const float in = std::min(kSmBytes, per_sm * ring / kLatency);
-    return kt * std::max(static_cast<float>(n) * w * kWTile / static_cast<float>(num_m) / kHbmBytes,
-                         per_sm * static_cast<float>(c.stage_bytes) / in);
-  };
   const float nt = static_cast<float>(plan.nt), split = static_cast<float>(plan.split);
+  const float stage = static_cast<float>(c.stage_bytes), mma = std::max(0.030f, nt / 2 / 1900);
+  auto round = [&](int64_t n) {  // us of n resident CTAs, up to their epilogues
+    const float per_sm = static_cast<float>(ceil_div(n, one));
+    const float busy = std::min(1.0f, static_cast<float>(n) / sms);
+    const float hbm = static_cast<float>(n) * w * kWTile / static_cast<float>(num_m) /
+                      (kHbmBytes * (0.3f + 0.7f * busy));
+    const float in = std::max(per_sm * stage / kSmBytes, stage * kLatency / ring);
+    const float issue = std::max(0.1f + 4 * w * mma, per_sm * 4 * w * mma);
+    return kt * std::max({hbm, in, issue});
+  };
   const float epilogue = plan.split == 1
                              ? nt * (g.gated ? 0.023f : 0.013f)
                              : 0.4f + w * nt * (0.030f + 0.020f / split);
+  // two CTAs on an SM: a fifth of an epilogue hides behind the other's
   const int64_t full = ctas / (one * occ), rest = ctas % (one * occ);
-  float us = 3.0f + static_cast<float>(full) * (round(one * occ) + epilogue);
-  if (rest > 0) us += round(rest) + epilogue;
+  float us = (c.bytes > 113 * 1024 ? 3.2f : 2.5f) + static_cast<float>(full) * (round(one * occ) + epilogue * (occ == 2 ? 1.8f : 1.0f));
+  if (rest > 0) us += round(rest) + epilogue * (rest > one ? 1.8f : 1.0f);
   return us;
 }
 
-Plan plan_of(const W8A8Args& g) {
+// An e4m3 MMA loses a part of its accumulator's last place at each step, always
+// towards zero: measured 4.5e-9 of the result a step of 32, 1e-6 after 7168 of
+// K. Where the output is fp32, no accumulator takes more than kPiece K tiles:
+// the K splits and pieces of a swap CTA are added up in fp32 instead. Against a
+// 16-bit output's rounding (2^-9 at best) the loss is nothing.
+constexpr int kPiece = 40;
+
+Plan search(const W8A8Args& g) {
   const int64_t k_tiles = ceil_div(g.K, kBK);
-  Plan best{true, 0, 1, false};
-  float least = g.M > 128 ? plan_us(best, g) : 1e30f;
+  const bool pieces = g.e4m3 && g.out_dtype == PK_F32;
+  Plan best{true, 0, 1, false, 1};
+  float least = g.M > 128 && !(pieces && k_tiles > kPiece) ? plan_us(best, g) : 1e30f;
+  int64_t fewest = 1ll << 60;  // K tiles over kPiece in an accumulator, 0 before all else
+  if (least < 1e30f) fewest = 0;
   // token tiles as even as sixteens allow, from as few as there can be to 16 wide
-  for (int64_t num_m = ceil_div(g.M, kMaxTokens), nt = 0, last = 0; num_m <= 16; ++num_m) {
+  for (int64_t num_m = ceil_div(g.M, kMaxTokens), nt = 0, last = 0; num_m <= ceil_div(g.M, 256) + 16;
+       ++num_m) {
     nt = ceil_div(ceil_div(g.M, num_m), 16) * 16;
     if (nt == last) continue;
     last = nt;
     for (int split = 1; split <= kMaxSplit && split <= k_tiles; split *= 2) {
       for (int deep = 0; deep < 2; ++deep) {
-        const Plan plan{false, static_cast<int>(nt), split, deep != 0};
+        Plan plan{false, static_cast<int>(nt), split, deep != 0, 1};
         if (!swap_smem(plan, g.gated, k_tiles).fits) continue;
+        const int64_t kt = ceil_div(k_tiles, split);
+        const int cols = plan.nt * (g.gated ? 2 : 1);
+        if (pieces)
+          while (plan.pieces * kPiece < kt && 2 * plan.pieces * cols <= (deep ? 512 : 256)) plan.pieces *= 2;
+        const int64_t over = pieces ? std::max<int64_t>(0, ceil_div(kt, plan.pieces) - kPiece) : 0;
         const float us = plan_us(plan, g);
-        if (us < least) {
+        if (over < fewest || (over == fewest && us < least)) {
+          fewest = over;
           least = us;
           best = plan;
         }
@@ -940,6 +991,26 @@ Plan plan_of(const W8A8Args& g) {
     if (nt == 16) break;
   }
   return best;
+}
+
+// The plans of recent sizes, per host thread (a decode loop asks for the same
+// few; a search is several microseconds): a function of the sizes alone.
+Plan plan_of(const W8A8Args& g) {
+  struct Entry {
+    int64_t M, N, K;
+    int key, sms;
+    Plan plan;
+  };
+  static thread_local Entry cache[64] = {};
+  const int key = 1 + (g.gated ? 2 : 0) + (g.e4m3 ? 4 : 0) + (g.out_dtype == PK_F32 ? 8 : 0);
+  const uint64_t hash = (static_cast<uint64_t>(g.M) * 0x9E3779B97F4A7C15ull ^
+                         static_cast<uint64_t>(g.N) * 0xC2B2AE3D27D4EB4Full ^
+                         static_cast<uint64_t>(g.K) * 0x165667B19E3779F9ull) + key;
+  Entry& e = cache[(hash ^ hash >> 32 ^ hash >> 17) & 63];
+  const int sms = num_sms();
+  if (e.M != g.M || e.N != g.N || e.K != g.K || e.key != key || e.sms != sms)
+    e = Entry{g.M, g.N, g.K, key, sms, search(g)};
+  return e.plan;
 }
 
 template <bool kE4M3, bool kGated>

@@ -87,6 +87,24 @@ def test_w8a8_gemm(M, N, K, code):
     assert pk.device_status() == (0, 0)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 512, 28672), (16, 256, 28672), (300, 300, 28672),
+                                   (600, 4096, 12000), (130, 130, 100000)])
+def test_long_e4m3_sums_keep_fp32_precision(M, N, K):
+    # no accumulator of an fp32 output takes more than 5120 of K, where a tensor
+    # core's truncation (half a last place of fp32 a step of 32, towards zero, is
+    # 2^-25 * 160 = 4.8e-6 at worst, and 4.5e-9 * 160 = 7e-7 of a sum of either
+    # sign as measured) stays below 1e-6 of the result's norm
+    for weights in (1, 2):
+        a, sa, w, _ = _operands(M, N, K, torch.float8_e4m3fn, seed=5, weights=weights)
+        ref = _product64(a, sa, w[0], w[1])[0]
+        if weights == 1:
+            y = pk.w8a8_gemm(a, sa, w[0], w[1])
+        else:
+            ref = _act64(ref, "silu")[0] * _product64(a, sa, w[2], w[3])[0]
+            y = pk.w8a8_gated_gemm(a, sa, *w)
+        assert (torch.linalg.norm(y.double() - ref) <= 1e-6 * weights * torch.linalg.norm(ref)).item()
+
+
 def _act64(g, act):
     if act == "silu":
         return g * torch.sigmoid(g), g
