@@ -19,7 +19,8 @@ from .gemm_int4 import (int4_gemm, int4_gemm_host, pack_int4_n, quantize_int4,  
 from .gemm_w8a8 import (dequantize_rows, quantize_rows, w8a8_gated_gemm,  # noqa: F401
                         w8a8_gemm)
 from .gptq import gptq_quantize_int4  # noqa: F401
-from .linear import W4A16Linear, quantize_linear_layers  # noqa: F401
+from .linear import (W4A16Linear, W8A8GatedMLP, W8A8Linear,  # noqa: F401
+                     quantize_linear_layers)
 from .norm import rms_norm_quant  # noqa: F401
 
 __version__ = "0.1.0"

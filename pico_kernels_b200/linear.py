@@ -1,4 +1,5 @@
-"""W4A16 ``nn.Linear`` drop-in over the packed-int4 GEMM.
+"""Quantized ``nn.Linear`` drop-ins: W4A16 over the packed-int4 GEMM, and W8A8
+over the 8-bit products (``W8A8Linear``, ``W8A8GatedMLP``, below).
 
 The reference quantizes the transformer's ``nn.Linear`` layers in place
 (quantize.py:124-129 selects them, quantize.py:160-184 swaps in fake-quant
@@ -16,8 +17,15 @@ keeps each layer's weight as packed int4 codes plus group scales and runs
   ``x``'s dtype, like ``nn.Linear``. M = 1 runs the CUDA-core GEMV, small M the
   tensor-core decode, large M the tcgen05 prefill path.
 
+``W8A8Linear`` holds the weight as 8-bit codes ``[out, in]`` (int8 or e4m3) with
+one scale per output channel and quantizes its input per token on every call;
+``W8A8GatedMLP`` runs a gated feed-forward block on such weights: norm with the
+residual's addition, both input projections with the activation and product in
+one kernel, and the output projection. Quantized weights take no gradient.
+
 ``quantize_linear_layers(model)`` swaps every (or every selected) ``nn.Linear``
-of a module tree for a ``W4A16Linear`` in place.
+of a module tree for a ``W4A16Linear`` (or, with ``scheme="w8a8"``, a
+``W8A8Linear``) in place.
 """
 
 from __future__ import annotations
@@ -29,8 +37,11 @@ import torch.nn as nn
 
 from . import _lib
 from .gemm_int4 import int4_gemm, quantize_int4_grouped
+from .gemm_w8a8 import (ACTIVATIONS, check_codes_dtype, dequantize_rows, quantize_rows, row_pitch,
+                        w8a8_gated_gemm, w8a8_gemm)
+from .norm import rms_norm_quant
 
-__all__ = ["W4A16Linear", "quantize_linear_layers"]
+__all__ = ["W4A16Linear", "W8A8Linear", "W8A8GatedMLP", "quantize_linear_layers"]
 
 
 class W4A16Linear(nn.Module):
@@ -133,6 +144,147 @@ class W4A16Linear(nn.Module):
                 f"bias={self.bias is not None}, group_size={self.group_size}, int4")
 
 
+class W8A8Linear(nn.Module):
+    """``y = x @ W^T + b`` with W in 8-bit codes, one scale per output channel,
+    and x quantized to the same 8-bit type per row (token) on every call."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 dtype: torch.dtype = torch.int8,
+                 device: torch.device | str | None = None) -> None:
+        super().__init__()
+        check_codes_dtype(dtype)
+        self.in_features = in_features
+        self.out_features = out_features
+        self.dtype = dtype
+        # rows padded to the pitch the kernels load: a view of them stays as laid
+        # out when the module moves between devices
+        self.register_buffer("codes", torch.zeros((out_features, row_pitch(in_features)),
+                                                  dtype=dtype, device=device))
+        self.register_buffer("scales", torch.zeros(out_features, dtype=torch.float32,
+                                                   device=device))
+        if bias:
+            self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32,
+                                                     device=device))
+        else:
+            self.bias = None
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, dtype: torch.dtype = torch.int8) -> "W8A8Linear":
+        """Quantize ``linear.weight`` (on a CUDA device) per output channel, to
+        int8 or ``torch.float8_e4m3fn``. The bias is kept in fp32."""
+        w = linear.weight.detach()
+        _lib.require_cuda(w)
+        layer = cls(linear.in_features, linear.out_features, linear.bias is not None, dtype,
+                    w.device)
+        codes, scales = quantize_rows(w, dtype)
+        layer.weight8.copy_(codes)
+        layer.scales.copy_(scales)
+        if linear.bias is not None:
+            layer.bias.copy_(linear.bias.detach().float())
+        return layer
+
+    @property
+    def weight8(self) -> torch.Tensor:
+        """The codes ``[out, in]`` (a view of their padded storage)."""
+        return self.codes[:, : self.in_features]
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise _lib.ShapeError(f"expected {self.in_features} input features, got {x.shape[-1]}")
+        codes, scale = quantize_rows(x.reshape(-1, self.in_features), self.dtype)
+        return self.product(codes, scale, x.dtype).reshape(*x.shape[:-1], self.out_features)
+
+    def product(self, codes: torch.Tensor, scale: torch.Tensor,
+                out_dtype: torch.dtype) -> torch.Tensor:
+        """The layer on inputs that are quantized already (``quantize_rows``,
+        ``rms_norm_quant``): ``codes[M, in]`` and ``scale[M]`` to ``[M, out]``."""
+        return w8a8_gemm(codes, scale, self.weight8, self.scales, bias=self.bias,
+                         out_dtype=out_dtype)
+
+    def dequantized_weight(self) -> torch.Tensor:
+        """fp32 ``W[out, in]`` the layer computes with (codes x channel scales)."""
+        return dequantize_rows(self.weight8, self.scales)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, {str(self.dtype).removeprefix('torch.')}")
+
+
+class W8A8GatedMLP(nn.Module):
+    """Gated feed-forward block on 8-bit weights:
+    ``down(act(gate(n)) * up(n))`` with ``n`` the block's input, or its RMS norm
+    when the block holds a norm weight.
+
+    Four launches a call: the norm (or the quantizer) that writes 8-bit rows, the
+    gated product, the quantizer of its result, and the output product.
+    """
+
+    def __init__(self, gate: W8A8Linear, up: W8A8Linear, down: W8A8Linear,
+                 norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 activation: str = "silu") -> None:
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise _lib.ShapeError(f"activation must be one of {', '.join(ACTIVATIONS)} "
+                                  f"(got {activation!r})")
+        if gate.bias is not None or up.bias is not None:
+            raise _lib.ShapeError("the gated product has no bias in its input projections")
+        if gate.in_features != up.in_features or gate.out_features != up.out_features:
+            raise _lib.ShapeError("gate and up must have the same sizes")
+        if down.in_features != gate.out_features:
+            raise _lib.ShapeError(f"down takes {down.in_features} features, the gated product "
+                                  f"gives {gate.out_features}")
+        if gate.dtype != up.dtype:
+            raise _lib.DtypeError("gate and up must have the same 8-bit type")
+        if norm_weight is not None and norm_weight.shape != (gate.in_features,):
+            raise _lib.ShapeError(f"norm_weight must be [{gate.in_features}] "
+                                  f"(got {tuple(norm_weight.shape)})")
+        self.gate, self.up, self.down = gate, up, down
+        self.eps = eps
+        self.activation = activation
+        self.register_buffer("norm_weight", norm_weight)
+
+    @classmethod
+    def from_linears(cls, gate: nn.Linear, up: nn.Linear, down: nn.Linear,
+                     norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                     activation: str = "silu",
+                     dtype: torch.dtype = torch.int8) -> "W8A8GatedMLP":
+        """Quantize the three projections (``W8A8Linear.from_linear``)."""
+        return cls(*(W8A8Linear.from_linear(m, dtype) for m in (gate, up, down)),
+                   norm_weight=None if norm_weight is None else norm_weight.detach(), eps=eps,
+                   activation=activation)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """``x[..., in]`` to ``[..., out]`` in ``x``'s type. With ``residual``
+        (blocks with a norm only) the norm is that of ``h = x + residual`` and
+        ``(output, h)`` is returned, ``h`` being the residual stream after it."""
+        if x.shape[-1] != self.gate.in_features:
+            raise _lib.ShapeError(f"expected {self.gate.in_features} input features, got "
+                                  f"{x.shape[-1]}")
+        if residual is not None and self.norm_weight is None:
+            raise _lib.ShapeError("a residual needs a block with a norm")
+        x2 = x.reshape(-1, x.shape[-1])
+        h = None
+        if self.norm_weight is None:
+            q, s = quantize_rows(x2, self.gate.dtype)
+        elif residual is None:
+            q, s = rms_norm_quant(x2, self.norm_weight, self.eps, dtype=self.gate.dtype)
+        else:
+            if residual.shape != x.shape:
+                raise _lib.ShapeError(f"residual must be {tuple(x.shape)} (got "
+                                      f"{tuple(residual.shape)})")
+            q, s, h = rms_norm_quant(x2, self.norm_weight, self.eps,
+                                     residual=residual.reshape(x2.shape), dtype=self.gate.dtype)
+        # the block's own type for the hidden values, which the quantizer reads next
+        y = w8a8_gated_gemm(q, s, self.gate.weight8, self.gate.scales, self.up.weight8,
+                            self.up.scales, activation=self.activation, out_dtype=x.dtype)
+        q, s = quantize_rows(y, self.down.dtype)
+        out = self.down.product(q, s, x.dtype).reshape(*x.shape[:-1], self.down.out_features)
+        return out if h is None else (out, h.reshape(x.shape))
+
+    def extra_repr(self) -> str:
+        return f"activation={self.activation}, norm={self.norm_weight is not None}"
+
+
 def _capture_inputs(model: nn.Module, module: nn.Module, calib) -> torch.Tensor:
     """Inputs ``module`` sees when ``model`` runs on ``calib`` (a tensor or a
     tuple of positional arguments), flattened to ``[rows, in]``
@@ -154,8 +306,11 @@ def _capture_inputs(model: nn.Module, module: nn.Module, calib) -> torch.Tensor:
 def quantize_linear_layers(model: nn.Module, group_size: int = 128,
                            select: Callable[[str, nn.Linear], bool] | None = None,
                            dtype: torch.dtype | None = None, calib=None,
-                           damp: float = 0.01, act_order: bool = False) -> nn.Module:
-    """Replace ``nn.Linear`` children in place with ``W4A16Linear``.
+                           damp: float = 0.01, act_order: bool = False, *,
+                           scheme: str = "w4a16") -> nn.Module:
+    """Replace ``nn.Linear`` children in place with ``W4A16Linear``, or with
+    ``scheme="w8a8"`` by ``W8A8Linear`` (``dtype`` then is the 8-bit type, int8 by
+    default; no groups, no calibration; any ``out_features``).
 
     ``select(name, module)`` picks the layers (default: every ``nn.Linear``
     with an even ``out_features``); quantize.py:124-129 picks those under
@@ -166,8 +321,15 @@ def quantize_linear_layers(model: nn.Module, group_size: int = 128,
     (the sequential re-capture of quantize.py:160-184); without it, per-group
     round-to-nearest. Returns ``model``.
     """
+    if scheme not in ("w4a16", "w8a8"):
+        raise _lib.ShapeError(f"scheme must be w4a16 or w8a8 (got {scheme!r})")
+    w8a8 = scheme == "w8a8"
+    if w8a8:
+        if calib is not None or act_order:
+            raise _lib.ShapeError("w8a8 rounds to nearest: no calibration, no act_order")
+        check_codes_dtype(torch.int8 if dtype is None else dtype)
     targets = [name for name, mod in model.named_modules()
-               if isinstance(mod, nn.Linear) and mod.out_features % 2 == 0
+               if isinstance(mod, nn.Linear) and (w8a8 or mod.out_features % 2 == 0)
                and (select is None or select(name, mod))]
     for name in targets:
         parent = model
@@ -175,6 +337,9 @@ def quantize_linear_layers(model: nn.Module, group_size: int = 128,
         for p in path:
             parent = getattr(parent, p)
         mod = getattr(parent, leaf)
+        if w8a8:
+            setattr(parent, leaf, W8A8Linear.from_linear(mod, torch.int8 if dtype is None else dtype))
+            continue
         x = _capture_inputs(model, mod, calib) if calib is not None else None
         setattr(parent, leaf, W4A16Linear.from_linear(mod, group_size, dtype, calib=x, damp=damp,
                                                       act_order=act_order and x is not None))

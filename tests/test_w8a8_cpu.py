@@ -168,3 +168,28 @@ def test_row_storage_and_layouts(as_if_on_a_gpu):
         assert torch.equal(r, v.reshape(-1, v.shape[-1])) and ld >= v.shape[-1]
         assert r.shape[0] == 1 or r.stride(0) == ld
         assert copied or r.data_ptr() == v.data_ptr()
+
+
+def test_modules_refuse():
+    S, D = _lib.ShapeError, _lib.DtypeError
+    def lin(i, o, bias=False, dtype=torch.int8):
+        return pk.W8A8Linear(i, o, bias, dtype)
+    a, down = lin(32, 64), lin(64, 32, True)
+    assert a.weight8.shape == (64, 32) and lin(17, 3).codes.shape == (3, 32)
+    pk.W8A8GatedMLP(a, a, down)
+    for err, call in [
+            (D, lambda: lin(32, 64, dtype=torch.uint8)),
+            (S, lambda: pk.W8A8GatedMLP(a, a, down, activation="relu")),
+            (S, lambda: pk.W8A8GatedMLP(lin(32, 64, True), a, down)),
+            (S, lambda: pk.W8A8GatedMLP(a, lin(32, 48), down)),
+            (S, lambda: pk.W8A8GatedMLP(a, a, lin(48, 32))),
+            (D, lambda: pk.W8A8GatedMLP(a, lin(32, 64, dtype=torch.float8_e4m3fn), down)),
+            (S, lambda: pk.W8A8GatedMLP(a, a, down, norm_weight=torch.ones(31))),
+            (D, lambda: pk.W8A8Linear.from_linear(torch.nn.Linear(4, 4))),
+            (S, lambda: pk.quantize_linear_layers(torch.nn.Linear(4, 4), scheme="w2a2")),
+            (S, lambda: pk.quantize_linear_layers(torch.nn.Linear(4, 4), scheme="w8a8",
+                                                  calib=torch.zeros(1, 4))),
+            (D, lambda: pk.quantize_linear_layers(torch.nn.Linear(4, 4), scheme="w8a8",
+                                                  dtype=torch.bfloat16))]:
+        with pytest.raises(err):
+            call()
