@@ -229,15 +229,22 @@ __device__ __forceinline__ Eight<W> load_weights(const W* w, int c0, int cols) {
   else return load_row8<W, true>(w, c0, cols);
 }
 
-// e + r, rounded to the stream's type.
+// e + r, rounded to the stream's type. Two 16-bit values at a time: the sum of
+// two such numbers is rounded once (the same bits as an fp32 addition and a
+// rounding: fp32 holds every sum in which both matter), in one instruction
+// where unpacking, adding and packing took seven.
 template <typename T>
 __device__ __forceinline__ void add(Eight<T>& e, const Eight<T>& r) {
-  float a[8], b[8];
-  e.values(a);
-  r.values(b);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] += b[j];
-  e.round(a);
+  for (int i = 0; i < Eight<T>::kWords; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      e.w[i] = __float_as_uint(__uint_as_float(e.w[i]) + __uint_as_float(r.w[i]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(e.w[i]) : "r"(e.w[i]), "r"(r.w[i]));
+    } else {
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(e.w[i]) : "r"(e.w[i]), "r"(r.w[i]));
+    }
+  }
 }
 
 template <typename T>
@@ -404,7 +411,8 @@ constexpr int kCtaThreads = 1024;  // threads an SM holds of it: 64 registers ea
 // start off a 16-byte boundary are copied as the aligned blocks that hold them
 // (each holds at least one of their values) and shifted when they are read.
 // Between the passes a thread holds u of its chunks (kHeld; rows of up to 16384
-// columns), or the first pass leaves h in the slot for the second.
+// columns) and its slot takes the next row at once (kEarly), or the first pass
+// leaves h in the slot for the second.
 //
 // kWhole: every row of every operand is whole 16-byte chunks. It is a
 // parameter of the kernel, not a test in it, because instructions set the
@@ -419,6 +427,7 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
   constexpr bool kNorm = kMode != kCodes;
   constexpr int kStreams = kMode == kSummed ? 2 : 1;
   constexpr int kSize = sizeof(T);
+  constexpr bool kEarly = kWhole && kHeld;  // a slot is free once its row has been read
   const int lanes = p.lanes, groups = blockDim.x / lanes;
   const int group = threadIdx.x / lanes, t = threadIdx.x % lanes;
   // Rows and strides are 32 bits here (the launcher sees to it): an address is
@@ -438,7 +447,16 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
   };
   auto copy_row = [&](const uint8_t* src, uint32_t slot) {
     const int bytes = p.cols * kSize;
-    if constexpr (kWhole) {
+    if constexpr (kEarly) {
+      const uint8_t* s = src + t * 8 * kSize;
+      uint32_t d = slot + t * 8 * kSize;
+      const int stride = lanes * 8 * kSize;
+#pragma unroll
+      for (int c = 0; c < kHold; ++c, s += stride, d += stride)
+        if ((c * lanes + t) * 8 < p.cols)
+#pragma unroll
+          for (int i = 0; i < kSize / 2; ++i) copy16_async(d + 16 * i, s + 16 * i);
+    } else if constexpr (kWhole) {
       for (int b = t * 8 * kSize; b < bytes; b += lanes * 8 * kSize)
 #pragma unroll
         for (int i = 0; i < kSize / 2; ++i) copy16_async(slot + b + 16 * i, src + b + 16 * i);
@@ -456,7 +474,7 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
     copy_commit();
   };
 
-  for (int s = 0; s + 1 < p.stages; ++s) fetch(first + s * step, s);
+  for (int s = 0; s + (kEarly ? 0 : 1) < p.stages; ++s) fetch(first + s * step, s);
   if constexpr (kNorm) {  // the weights towards L1, where all rows of the SM read them
     const int wsize = p.weight_f32 ? 4 : kSize;
     for (int c0 = t * 8; c0 < p.cols; c0 += lanes * 8)
@@ -469,8 +487,10 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
   for (uint32_t base = blockIdx.x * groups; base < rows; base += step) {
     const uint32_t row = base + group;
     const bool live = row < rows;
-    fetch(row + (p.stages - 1) * step, stage == 0 ? p.stages - 1 : stage - 1);
-    if (p.stages == 2) copy_wait<1>();
+    if constexpr (!kEarly)
+      fetch(row + (p.stages - 1) * step, stage == 0 ? p.stages - 1 : stage - 1);
+    if (p.stages == 1) copy_wait<0>();
+    else if (p.stages == 2) copy_wait<1>();
     else copy_wait<3>();
     if constexpr (!kWhole) group_sync(lanes);
     const uint32_t slot = slots + stage * kStreams * p.slot;
@@ -484,6 +504,10 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
     // a whole row's slot where it is read again; another adds again).
     auto chunk = [&](int c0, auto start) {
       constexpr bool kStart = decltype(start)::value;
+      if constexpr (kEarly && !kStart) {  // the slot holds a later row by now
+        const uint8_t* from = kMode == kSummed ? at(p.h, row, p.sh) : at(p.x, row, p.sx);
+        return load8<T, false>(reinterpret_cast<const T*>(from) + c0);
+      }
       Eight<T> e = staged8<T, kWhole>(slot + off + c0 * kSize);
       if constexpr (kMode == kSummed && (kStart || kHeld || !kWhole)) {
         add<T>(e, staged8<T, kWhole>(slot + p.slot + offr + c0 * kSize));
@@ -551,6 +575,7 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
           big = largest(big, held[c]);
         }
       }
+      if constexpr (kEarly) fetch(row + p.stages * step, stage);
     } else {
 #pragma unroll 2
       for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
@@ -654,22 +679,28 @@ __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams 
   }
 }
 
-// Eight codes (two words) times the row's scale.
-template <typename T>
-__device__ __forceinline__ Eight<T> code_values(uint32_t w0, uint32_t w1, bool e4m3, float s) {
+// Eight codes (two words) times the row's scale. An int8 code becomes a float by
+// byte selection: with its sign bit flipped it is the low byte of 2^23 + 128 +
+// code, whose excess one exact subtraction takes off (the conversion
+// instruction runs at a quarter of their rate).
+template <typename T, bool kE4M3>
+__device__ __forceinline__ Eight<T> code_values(uint32_t w0, uint32_t w1, float s) {
   float v[8];
+  if constexpr (kE4M3) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const uint32_t pair = (j < 4 ? w0 : w1) >> (8 * (j & 2));
-    if (e4m3) {
+    for (int j = 0; j < 8; j += 2) {
+      const uint32_t pair = (j < 4 ? w0 : w1) >> (8 * (j & 2));
       const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair & 0xffffu),
                                                  __NV_E4M3));
       const float2 f = __half22float2(h);
       v[j] = f.x * s;
       v[j + 1] = f.y * s;
-    } else {
-      v[j] = static_cast<float>(static_cast<int8_t>(pair)) * s;
-      v[j + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8)) * s;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t flipped = (j < 4 ? w0 : w1) ^ 0x80808080u;
+      v[j] = (__uint_as_float(prmt(flipped, 0x4b000000u, 0x7540 | (j & 3))) - 8388736.0f) * s;
     }
   }
   Eight<T> e;
@@ -677,16 +708,16 @@ __device__ __forceinline__ Eight<T> code_values(uint32_t w0, uint32_t w1, bool e
   return e;
 }
 
-// kWhole: sixteen codes a thread, one 16-byte load (4096 x 8192 to bf16: 15.7
-// us, with eight 23.6). Else eight: rows of values that start off a 16-byte
+// kWhole: 32 bytes of values a thread (eight codes to fp32, sixteen to 16 bits). Else eight: rows of values that start off a 16-byte
 // boundary (odd widths) begin with up to seven single values (item 0), so that
 // the chunks after them store whole; their codes then start at any byte, and
 // come from the words that hold them (1000 x 5001: 5.7 us, by bytes 21.5).
-template <typename T, bool kWhole>
+template <typename T, bool kE4M3, bool kWhole>
 __global__ void __launch_bounds__(256)
     dequantize_rows_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                            const float* __restrict__ scale, T* __restrict__ out, int64_t ldo,
-                           int64_t rows, int cols, int e4m3) {
+                           int64_t rows, int cols) {
+  constexpr int kPer = sizeof(T) == 4 ? 8 : 16;
   griddep_wait();
   griddep_launch_dependents();
   const int item = blockIdx.x * blockDim.x + threadIdx.x;
@@ -695,12 +726,17 @@ __global__ void __launch_bounds__(256)
     const uint8_t* src = q + row * ldq;
     T* dst = out + row * ldo;
     if constexpr (kWhole) {
-      const int c0 = item * 16;
+      const int c0 = item * kPer;
       if (c0 >= cols) continue;
       const float s = scale[row];
-      const uint4 w = __ldcg(reinterpret_cast<const uint4*>(src + c0));
-      store8<T>(dst + c0, code_values<T>(w.x, w.y, e4m3, s));
-      store8<T>(dst + c0 + 8, code_values<T>(w.z, w.w, e4m3, s));
+      if constexpr (kPer == 8) {
+        const uint2 w = __ldcg(reinterpret_cast<const uint2*>(src + c0));
+        store8<T>(dst + c0, code_values<T, kE4M3>(w.x, w.y, s));
+      } else {
+        const uint4 w = __ldcg(reinterpret_cast<const uint4*>(src + c0));
+        store8<T>(dst + c0, code_values<T, kE4M3>(w.x, w.y, s));
+        store8<T>(dst + c0 + 8, code_values<T, kE4M3>(w.z, w.w, s));
+      }
       continue;
     }
     const int head =
@@ -723,7 +759,7 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < 8; ++j)
         if (c0 + j < c1) w[j >> 2] |= static_cast<uint32_t>(src[c0 + j]) << (8 * (j & 3));
     }
-    const Eight<T> e = code_values<T>(w[0], w[1], e4m3, s);
+    const Eight<T> e = code_values<T, kE4M3>(w[0], w[1], s);
     if (c1 - c0 == 8) {
       store8<T>(dst + c0, e);
     } else {
@@ -803,8 +839,12 @@ cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
   // a chunk past an unaligned row's last block is read (and discarded)
   const int64_t cols8 = static_cast<int64_t>(p.cols + 7) / 8 * 8;
   const int64_t slot = cols8 * kSize + (chunks ? 0 : 32);
+  const int64_t streams = residual ? 2 : 1;
   p.stages = p.lanes == 32 ? 4 : 2;
-  const int64_t bytes = slot * (residual ? 2 : 1) * groups * p.stages;
+  if (chunks && p.cols <= kHold * 8 * kMaxLanes && p.lanes > 32 &&
+      (slot * streams * 2 + 1536) * (kCtaThreads / threads) > 228 * 1024)
+    p.stages = 1;  // as many CTAs as the registers allow before a second row in flight
+  const int64_t bytes = slot * streams * groups * p.stages;
   const int64_t widest = std::max({p.ldx, p.ldr, p.ldh, p.ldq}) * kSize;
   p.sx = static_cast<uint32_t>(p.ldx * kSize);
   p.sr = static_cast<uint32_t>(p.ldr * kSize);
@@ -838,7 +878,7 @@ cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* 
   const bool whole = cols % 16 == 0 && aligned16(q) && ldq % 16 == 0 && aligned16(out) &&
                      (ldo * sizeof(T)) % 16 == 0;
   // one item more for the start of an unaligned row
-  const int items = whole ? cols / 16 : (cols + 7) / 8 + 1;
+  const int items = whole ? cols / (sizeof(T) == 4 ? 8 : 16) : (cols + 7) / 8 + 1;
   int tx = 32;
   while (tx < 256 && tx < items) tx *= 2;
   const int ty = 256 / tx;
@@ -846,10 +886,12 @@ cudaError_t launch_dequantize_typed(const uint8_t* q, int64_t ldq, const float* 
   const dim3 grid(static_cast<unsigned>((items + tx - 1) / tx),
                   static_cast<unsigned>(gy < 65535 ? gy : 65535));
   const dim3 block(tx, ty);
-  return whole ? launch_chained(dequantize_rows_kernel<T, true>, grid, block, 0, s, q, ldq, scale,
-                                out, ldo, rows, cols, e4m3)
-               : launch_chained(dequantize_rows_kernel<T, false>, grid, block, 0, s, q, ldq, scale,
-                                out, ldo, rows, cols, e4m3);
+  auto go = [&](auto kernel) {
+    return launch_chained(kernel, grid, block, 0, s, q, ldq, scale, out, ldo, rows, cols);
+  };
+  if (e4m3)
+    return whole ? go(dequantize_rows_kernel<T, true, true>) : go(dequantize_rows_kernel<T, true, false>);
+  return whole ? go(dequantize_rows_kernel<T, false, true>) : go(dequantize_rows_kernel<T, false, false>);
 }
 
 }  // namespace

@@ -48,7 +48,9 @@ struct Params {
   int split, nt, stages, stage_bytes, tmem_cols, own_red;
   int pieces;        // swap: accumulators that a CTA's K range is summed in
   int num_m, num_n;  // tiles
-  int whole;         // pair: units that are whole tiles; each later tile is two half-width units
+  // pair: units that are whole tiles; each later tile is `parts` narrower units
+  int whole, parts;
+  int box;           // pair: channels of a TMA box (32 where there are quarter units, else 64)
   int* status;
 };
 
@@ -460,8 +462,7 @@ __global__ void __launch_bounds__(kThreads)
 // ---------------------------------------------------------------------------
 struct PairCfg {
   static constexpr int kATile = 128 * kBK;  // this CTA's 128 tokens
-  static constexpr int kBTile = 128 * kBK;  // this CTA's 128 channels, two boxes of 64
-  static constexpr int kBBox = 64 * kBK;
+  static constexpr int kBTile = 128 * kBK;  // this CTA's 128 channels
   static constexpr int kStageBytes = kATile + kBTile;
   static constexpr int kStages = 6;
   static constexpr int kBarOff = kStages * kStageBytes;
@@ -475,13 +476,16 @@ struct PairCfg {
 
 constexpr int kGroupM = 8;
 
-// Unit u of the schedule: tile (tm, tn), and half -1 (whole), 0 or 1.
-__device__ __forceinline__ void pair_unit(int u, const Params& p, int& tm, int& tn, int& half) {
+// Unit u of the schedule: tile (tm, tn), in how many parts, which part.
+__device__ __forceinline__ void pair_unit(int u, const Params& p, int& tm, int& tn, int& parts,
+                                          int& part) {
   int t = u;
-  half = -1;
+  parts = 1;
+  part = 0;
   if (u >= p.whole) {
-    t = p.whole + ((u - p.whole) >> 1);
-    half = (u - p.whole) & 1;
+    parts = p.parts;
+    t = p.whole + (u - p.whole) / parts;
+    part = (u - p.whole) % parts;
   }
   // rows of tiles in groups, so that the tiles in flight share operands in L2
   const int per_group = kGroupM * p.num_n;
@@ -513,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int rank = static_cast<int>(cluster_ctarank());
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int k_tiles = (p.K + kBK - 1) / kBK;
-  const int num_units = p.whole + 2 * (p.num_m * p.num_n - p.whole);
+  const int num_units = p.whole + p.parts * (p.num_m * p.num_n - p.whole);
   constexpr int kTileN = kGated ? 128 : 256;  // outputs of a tile
 
   if (warp == kTmaWarp && lane == 0) {
@@ -545,14 +549,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     int st = 0;
     uint32_t parity = 1;
     for (int u = pair; u < num_units && !fail; u += npairs) {
-      int tm, tn, half;
-      pair_unit(u, p, tm, tn, half);
+      int tm, tn, parts, at;
+      pair_unit(u, p, tm, tn, parts, at);
       const int row = tm * 256 + rank * 128;
-      // whole: 128 channels in two boxes; half: 64 of the half's outputs
-      const int boxes = half < 0 ? 2 : 1;
-      const int col = tn * kTileN + (kGated ? (half < 0 ? 0 : half * 64)
-                                            : (half < 0 ? rank * 128 : half * 128 + rank * 64));
-      const uint32_t tx = 2u * (C::kATile + boxes * C::kBBox);
+      // this CTA's 128 / parts channels: of gate or up, or its half of the outputs
+      const int boxes = 128 / parts / p.box;
+      const int col = tn * kTileN + at * (kTileN / parts) + (kGated ? 0 : rank * (128 / parts));
+      const uint32_t tx = 2u * (C::kATile + 128 / parts * kBK);
       for (int kt = 0; kt < k_tiles; ++kt) {
         fail = __any_sync(0xffffffffu, !mbar_wait(&empty[st], parity, p.status, kSiteW8PairProducer));
         if (fail) break;
@@ -562,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rank == 0) mbar_arrive_expect_tx(&full[st], tx);
           tma_load_2d_pair(base, &tmA, bar, kt * kBK, row);
           for (int b = 0; b < boxes; ++b)
-            tma_load_2d_pair(base + C::kATile + b * C::kBBox, tmW, bar, kt * kBK, col + b * 64);
+            tma_load_2d_pair(base + C::kATile + b * p.box * kBK, tmW, bar, kt * kBK, col + b * p.box);
         }
         __syncwarp();
         if (++st == C::kStages) {
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int local = 0, st = 0;
       uint32_t parity = 0;
       for (int u = pair; u < num_units && !fail; u += npairs, ++local) {
-        const uint32_t idesc = u < p.whole ? idesc8(kE4M3, 256, 256) : idesc8(kE4M3, 256, 128);
+        const uint32_t idesc = idesc8(kE4M3, 256, u < p.whole ? 256 : 256 / p.parts);
         const int ab = local & 1;
         if (local >= 2)
           fail = __any_sync(0xffffffffu, !mbar_wait_cluster(&acc_empty[ab], ((local >> 1) - 1) & 1,
@@ -610,16 +613,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- epilogue (both CTAs): a thread holds one token's row ----
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const int part = (warp - kEpiWarp0) >> 2;  // which half of the unit's outputs
+    const int part = (warp - kEpiWarp0) >> 2;  // which of two 32-output runs
     const int et = tid - kEpiWarp0 * 32;
     const uint32_t acc_empty0 = cluster_map(smem_u32(&acc_empty[0]), 0);
     int local = 0;
     for (int u = pair; u < num_units && !fail; u += npairs, ++local) {
-      int tm, tn, half;
-      pair_unit(u, p, tm, tn, half);
+      int tm, tn, parts, at;
+      pair_unit(u, p, tm, tn, parts, at);
       const int ab = local & 1;
-      const int outs = half < 0 ? kTileN : kTileN / 2;  // outputs of this unit
-      const int n0 = tn * kTileN + (half > 0 ? kTileN / 2 : 0);
+      const int outs = kTileN / parts;  // outputs of this unit
+      const int n0 = tn * kTileN + at * outs;
       // this unit's channel scales (gate then up) and bias
       float* sc = s_scale + ab * 256;
       float* bs = s_bias + ab * 256;
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * C::kAccCols;
 #pragma unroll 1
-      for (int c = part * (outs / 2); c < (part + 1) * (outs / 2); c += 32) {
+      for (int c = part * 32; c < outs; c += 64) {
         uint32_t x[32], y[32];
         tmem_ld_32x32b_x32(taddr + c, x);
         if (kGated) tmem_ld_32x32b_x32(taddr + outs + c, y);
@@ -868,26 +871,32 @@ cudaError_t launch_swap(const W8A8Args& g, const Plan& plan, cudaStream_t s, con
                 s, tm, p);
 }
 
+// A partial wave (the last, or all there is) runs as narrower units, two or four
+// a tile, where they still fit one wave: a half unit takes 0.75 of a tile's
+// time, a quarter 0.55.
+void pair_schedule(int64_t tiles, int slots, int* whole, int* parts) {
+  const int64_t tail = tiles % slots;
+  *parts = tail == 0 ? 1 : 4 * tail <= slots ? 4 : 2 * tail <= slots ? 2 : 1;
+  *whole = static_cast<int>(*parts == 1 ? tiles : tiles - tail);
+}
+
 template <bool kE4M3, bool kGated>
 cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
-  CUtensorMap tm[3];
-  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, 128, why) ||
-      !rows_map(&tm[1], g.w[0], g.N, g.K, g.ldw[0], 64, why))
-    return cudaErrorInvalidValue;
-  tm[2] = tm[1];
-  if (kGated && !rows_map(&tm[2], g.w[1], g.N, g.K, g.ldw[1], 64, why))
-    return cudaErrorInvalidValue;
   Params p = params_of(g);
   p.num_m = static_cast<int>(ceil_div(g.M, 256));
   p.num_n = static_cast<int>(ceil_div(g.N, kGated ? 128 : 256));
   const int tiles = p.num_m * p.num_n;
   const int slots = num_sms() / 2;
-  // A partial last wave whose halves still fit one wave runs as half-width
-  // units: about half a tile's time instead of a whole one's.
-  p.whole = tiles;
-  const int tail = tiles % slots;
-  if (tiles > slots && tail > 0 && 2 * tail <= slots) p.whole = tiles - tail;
-  const int units = p.whole + 2 * (tiles - p.whole);
+  pair_schedule(tiles, slots, &p.whole, &p.parts);
+  p.box = p.parts == 4 ? 32 : 64;
+  CUtensorMap tm[3];
+  if (!rows_map(&tm[0], g.a, g.M, g.K, g.lda, 128, why) ||
+      !rows_map(&tm[1], g.w[0], g.N, g.K, g.ldw[0], p.box, why))
+    return cudaErrorInvalidValue;
+  tm[2] = tm[1];
+  if (kGated && !rows_map(&tm[2], g.w[1], g.N, g.K, g.ldw[1], p.box, why))
+    return cudaErrorInvalidValue;
+  const int units = p.whole + p.parts * (tiles - p.whole);
   return launch(w8a8_pair_kernel<kE4M3, kGated>, 2 * (units < slots ? units : slots),
                 kThreads, 2, PairCfg::kSmem, s, tm, p);
 }
@@ -904,7 +913,8 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
 //  * swap: 2.5 us of launch and first loads, 0.7 more where a CTA takes most of an
 //    SM's memory (the next kernel's CTAs then wait for it); per token of a tile 13 ns of epilogue
 //    (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
-//  * pair: 6 us around the main loop, 0.28 us a K tile (0.21 of a half unit).
+//  * pair: 6 us around the main loop, 0.28 us a K tile (0.21 of a half unit, 0.155
+//    of a quarter).
 constexpr float kSmBytes = 150e3f, kHbmBytes = 6.3e6f, kLatency = 1.6f;  // per us; us
 
 float plan_us(const Plan& plan, const W8A8Args& g) {
@@ -913,13 +923,16 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
   const int64_t k_tiles = ceil_div(g.K, kBK);
   if (plan.pair) {
     const int64_t num_m = ceil_div(g.M, 256), tiles = num_m * ceil_div(g.N, g.gated ? 128 : 256);
-    const int64_t slots = num_sms() / 2, tail = tiles % slots;
+    const int slots = num_sms() / 2;
+    int whole, parts;
+    pair_schedule(tiles, slots, &whole, &parts);
     const float kt = static_cast<float>(k_tiles), weights = 256.0f * kBK / static_cast<float>(num_m);
     auto wave = [&](int64_t units, float k_tile_us) {
       return kt * std::max(static_cast<float>(units) * weights / kHbmBytes, k_tile_us);
     };
-    float us = 6.0f + static_cast<float>(tiles / slots) * wave(slots, 0.28f);
-    if (tail > 0) us += wave(tail, tiles > slots && 2 * tail <= slots ? 0.21f : 0.28f);
+    float us = 6.0f + static_cast<float>(whole / slots) * wave(slots, 0.28f);
+    if (tiles % slots > 0)
+      us += wave(tiles % slots, parts == 4 ? 0.155f : parts == 2 ? 0.21f : 0.28f);
     return us;
   }
   const SwapSmem c = swap_smem(plan, g.gated, k_tiles);
