@@ -708,6 +708,12 @@ int check_rows8(int64_t M, int64_t K, int q_dtype) {
   return PK_OK;
 }
 
+// Pointers at their element's boundary (elements of 1, 2 or 4 bytes).
+bool at_element(const void* p, int dtype) {
+  const uintptr_t size = dtype == PK_F32 ? 4 : is16(dtype) ? 2 : 1;
+  return reinterpret_cast<uintptr_t>(p) % size == 0;
+}
+
 // int32 holds K products of magnitude up to 2^14
 constexpr int64_t kMaxInt8K = (1ll << 17) - 1;
 
@@ -734,9 +740,10 @@ int run_w8a8(W8A8Args& g, int dtype, cudaStream_t s) {
     if ((reinterpret_cast<uintptr_t>(g.w[i]) & 15) || g.ldw[i] % 16 != 0)
       return fail(PK_ERR_ALIGN, "weights must be 16-byte aligned with a leading dimension of 16 k");
   }
-  const uintptr_t elt = g.out_dtype == PK_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(g.out) % elt != 0)
-    return fail(PK_ERR_ALIGN, "output must be aligned to its element");
+  if (!at_element(g.out, g.out_dtype) || !at_element(g.a_scale, PK_F32) ||
+      !at_element(g.w_scale[0], PK_F32) || !at_element(g.w_scale[1], PK_F32) ||
+      !at_element(g.bias, PK_F32))
+    return fail(PK_ERR_ALIGN, "output, scales and bias must be aligned to their elements");
   g.e4m3 = dtype == PK_E4M3;
   g.status = device_status_ptr();
   const char* why = "";
@@ -1061,6 +1068,8 @@ int pk_quantize_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx
   if (ldx < K || ldq < K) return fail(PK_ERR_SHAPE, "leading dimension too small");
   if (!is16(dtype) && dtype != PK_F32)
     return fail(PK_ERR_DTYPE, "quantize_rows takes f16, bf16 or f32");
+  if (!at_element(x, dtype) || !at_element(scale, PK_F32))
+    return fail(PK_ERR_ALIGN, "operands must be aligned to their elements");
   cudaError_t e = launch_quantize_rows(x, dtype, M, K, ldx, q, q_dtype == PK_E4M3, ldq, scale,
                                        as_stream(stream));
   if (e != cudaSuccess) return cuda_fail(e, "quantize_rows launch");
@@ -1076,6 +1085,8 @@ int pk_dequantize_rows(const void* q, int q_dtype, int64_t M, int64_t K, int64_t
   if (ldq < K || ldo < K) return fail(PK_ERR_SHAPE, "leading dimension too small");
   if (!is16(out_dtype) && out_dtype != PK_F32)
     return fail(PK_ERR_DTYPE, "dequantize_rows writes f16, bf16 or f32");
+  if (!at_element(out, out_dtype) || !at_element(scale, PK_F32))
+    return fail(PK_ERR_ALIGN, "operands must be aligned to their elements");
   cudaError_t e = launch_dequantize_rows(q, q_dtype == PK_E4M3, M, K, ldq, scale, out, out_dtype,
                                          ldo, as_stream(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dequantize_rows launch");
@@ -1099,6 +1110,9 @@ int pk_rms_norm_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ld
     return fail(PK_ERR_DTYPE, "the norm weight must be f32 or of x's type");
   if (!(eps >= FLT_MIN) || !(eps <= FLT_MAX))
     return fail(PK_ERR_SHAPE, "eps must be a finite normal fp32 number > 0");
+  if (!at_element(x, dtype) || !at_element(residual, dtype) || !at_element(h, dtype) ||
+      !at_element(weight, w_dtype) || !at_element(scale, PK_F32))
+    return fail(PK_ERR_ALIGN, "operands must be aligned to their elements");
   cudaError_t e = launch_rms_norm_quant(x, dtype, M, K, ldx, residual, ldr, weight,
                                         w_dtype == PK_F32, eps, h, ldh, q, q_dtype == PK_E4M3, ldq,
                                         scale, as_stream(stream));

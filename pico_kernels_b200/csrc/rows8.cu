@@ -33,7 +33,7 @@ namespace {
 constexpr float kTiny = 1e-12f;     // smallest row maximum, as in the int4 group scales
 constexpr uint32_t kInfBits = 0x7f800000u;
 constexpr int kMaxLanes = 512;      // threads of a row
-constexpr int64_t kMostStaged = 225 * 1024;  // shared memory for rows in flight
+constexpr int kMostStaged = 225 * 1024;  // shared memory for rows in flight
 
 struct RowsParams {
   const void* x;
@@ -776,7 +776,7 @@ template <typename... P, typename... A>
 cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t s,
                            A... args) {
   if (smem > 40 * 1024) {  // 48 KB less the static arrays need no attribute
-    const cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), smem);
+    const cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), kMostStaged);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

@@ -74,6 +74,13 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// After a wait that ran out: time (~100 us) for the copies and MMAs already
+// issued to end before the CTA's shared and tensor memory are released.
+__device__ __noinline__ void drain() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 200000) __nanosleep(1000);
+}
+
 template <bool kE4M3>
 __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                       uint32_t acc) {
@@ -238,7 +245,6 @@ __global__ void __launch_bounds__(kThreads)
   griddep_launch_dependents();
 
   bool fail = false;
-  int issued = 0;
   if (warp == kTmaWarp) {
     uint8_t* base = smem;
     uint64_t* bar = full;
@@ -253,7 +259,6 @@ __global__ void __launch_bounds__(kThreads)
         tma_load_2d(base + kW * kWTile, &tmA, bar, kt * kBK, m0);
       }
       __syncwarp();
-      ++issued;
       base += stage_bytes;
       if (++bar == empty) {
         bar = full;
@@ -447,12 +452,8 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 
-  if (fail && warp == kTmaWarp && lane == 0) {
-    // copies already issued land before the CTA's shared memory is released
-    for (int s = 0; s < issued; ++s) mbar_wait(&full[s % stages], (s / stages) & 1, nullptr, 0);
-  }
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(fail)) drain();
   if (warp == kMmaWarp) tmem_dealloc(tmem, p.tmem_cols);
 }
 
@@ -748,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(fail)) drain();
   cluster_sync();  // neither CTA leaves while the other may still touch its memory
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc_pair(tmem, 512);
@@ -785,10 +786,13 @@ Params params_of(const W8A8Args& g) {
   return p;
 }
 
+constexpr int kMaxSmem = 226 * 1024;
+
 template <typename Kernel>
 cudaError_t launch(Kernel kernel, int grid, int threads, int cluster, int smem, cudaStream_t s,
                    const CUtensorMap (&tm)[3], const Params& p) {
-  cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), smem);
+  // the attribute once and for all sizes (a plan's size changes from call to call)
+  cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), kMaxSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attrs[2];
@@ -829,7 +833,7 @@ SwapSmem swap_smem(const Plan& plan, bool gated, int64_t k_tiles) {
   c.own_red = sums > 0 && sums <= 16 * 1024;
   const int rest = kMaxTokens * 4 + kSwapBars + (c.own_red ? sums : 0) + 1024;
   // two CTAs an SM where half the memory holds four stages
-  const int half = 113 * 1024 - rest, whole = 226 * 1024 - rest;
+  const int half = kMaxSmem / 2 - rest, whole = kMaxSmem - rest;
   c.stages = (!plan.deep && half / c.stage_bytes >= 4 ? half : whole) / c.stage_bytes;
   c.stages = static_cast<int>(std::min<int64_t>(std::min(c.stages, 12), ceil_div(k_tiles, plan.split)));
   // sums without memory of their own go into the drained ring
@@ -885,6 +889,7 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
   Params p = params_of(g);
   p.num_m = static_cast<int>(ceil_div(g.M, 256));
   p.num_n = static_cast<int>(ceil_div(g.N, kGated ? 128 : 256));
+  if (static_cast<int64_t>(p.num_m) * p.num_n >= 1 << 29) return cudaErrorInvalidConfiguration;
   const int tiles = p.num_m * p.num_n;
   const int slots = num_sms() / 2;
   pair_schedule(tiles, slots, &p.whole, &p.parts);
@@ -936,7 +941,7 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
     return us;
   }
   const SwapSmem c = swap_smem(plan, g.gated, k_tiles);
-  const int occ = c.bytes <= 113 * 1024 ? 2 : 1;
+  const int occ = c.bytes <= kMaxSmem / 2 ? 2 : 1;
   const int64_t num_m = ceil_div(g.M, plan.nt);
   const int64_t ctas = num_m * ceil_div(g.N, 128) * plan.split;
   const float part = plan.split == 8 ? 120.0f / 148 : plan.split == 4 ? 132.0f / 148 : 1.0f;
@@ -959,7 +964,7 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
                              : 0.4f + w * nt * (0.030f + 0.020f / split);
   // two CTAs on an SM: a fifth of an epilogue hides behind the other's
   const int64_t full = ctas / (one * occ), rest = ctas % (one * occ);
-  float us = (c.bytes > 113 * 1024 ? 3.2f : 2.5f) + static_cast<float>(full) * (round(one * occ) + epilogue * (occ == 2 ? 1.8f : 1.0f));
+  float us = (c.bytes > kMaxSmem / 2 ? 3.2f : 2.5f) + static_cast<float>(full) * (round(one * occ) + epilogue * (occ == 2 ? 1.8f : 1.0f));
   if (rest > 0) us += round(rest) + epilogue * (rest > one ? 1.8f : 1.0f);
   return us;
 }

@@ -22,6 +22,7 @@ def test_c_abi_refuses_rows():
         assert call(**kw) == _lib.PK_ERR_SHAPE, kw
     for kw in (dict(dtype=I8), dict(q_dtype=BF), dict(q_dtype=_lib.PK_U8)):
         assert call(**kw) == _lib.PK_ERR_DTYPE, kw
+    assert call(x=65) == call(scale=66) == _lib.PK_ERR_ALIGN
     deq = dict(q=64, q_dtype=E4, M=4, K=100, ldq=112, scale=64, out=64, out_dtype=BF, ldo=100,
                stream=None)
 
@@ -47,6 +48,8 @@ def test_c_abi_refuses_norms():
         assert call(**kw) == _lib.PK_ERR_SHAPE, kw
     for kw in (dict(dtype=I8), dict(w_dtype=_lib.PK_F16), dict(q_dtype=F32)):
         assert call(**kw) == _lib.PK_ERR_DTYPE, kw
+    for kw in (dict(x=65), dict(residual=65), dict(h=65), dict(weight=65), dict(scale=66)):
+        assert call(**kw) == _lib.PK_ERR_ALIGN, kw
 
 
 @pytest.mark.parametrize("gated", [False, True])
@@ -68,7 +71,8 @@ def test_c_abi_refuses_products(gated):
         assert call(**kw) == _lib.PK_ERR_SHAPE, kw
     for kw in (dict(dtype=BF), dict(dtype=_lib.PK_U8), dict(out_dtype=I8), dict(out_dtype=E4)):
         assert call(**kw) == _lib.PK_ERR_DTYPE, kw
-    align = [dict(a=72), dict(w=65), dict(lda=104), dict(ldw=120), dict(out=65)]
+    align = [dict(a=72), dict(w=65), dict(lda=104), dict(ldw=120), dict(out=65), dict(sa=66),
+             dict(sw=66)]
     for kw in align + ([dict(u=72), dict(ldu=104)] if gated else []):
         assert call(**kw) == _lib.PK_ERR_ALIGN, kw
     assert _lib.last_error() != ""
