@@ -7,8 +7,8 @@
 //                 y_k = h_k * r * w_k, quantized as above
 //   dequantize    x_k = q_k * scale
 //
-// All three are bound by HBM: a row is read once, kept in registers while its
-// sum and its largest magnitude are reduced, and written once. The norm needs
+// All three are bound by HBM: a row is read once, kept while its sum and its
+// largest magnitude are reduced, and written once. The norm needs
 // one reduction, not two (the sum for r, then the maximum of y): r multiplies
 // the whole row, so the codes of y are those of u_k = h_k * w_k, and the sum of
 // h^2 and the maximum of |u| are reduced together; r enters the scale alone.
@@ -320,8 +320,19 @@ __device__ __forceinline__ float warp_sum(float v) {
 template <bool kNorm>
 __device__ __forceinline__ void reduce_row(int lanes, float& sum, float big, uint32_t& most,
                                            float* s_sum, uint32_t* s_max) {
+  most = __float_as_uint(big);
+  if (lanes < 32) {  // several rows in a warp: each among its own lanes
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      if (o < lanes) {
+        if constexpr (kNorm) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+    }
+    return;
+  }
   if constexpr (kNorm) sum = warp_sum(sum);
-  most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+  most = __reduce_max_sync(0xffffffffu, most);
   if (lanes == 32) return;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x % lanes) >> 5, warps = lanes >> 5;
   if (lane == 0) {
@@ -371,7 +382,7 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 __device__ __forceinline__ void group_sync(int lanes) {
-  if (lanes == 32) __syncwarp();
+  if (lanes <= 32) __syncwarp();
   else __syncthreads();
 }
 
@@ -475,15 +486,17 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
   };
 
   for (int s = 0; s + (kEarly ? 0 : 1) < p.stages; ++s) fetch(first + s * step, s);
-  if constexpr (kNorm) {  // the weights towards L1, where all rows of the SM read them
-    const int wsize = p.weight_f32 ? 4 : kSize;
-    for (int c0 = t * 8; c0 < p.cols; c0 += lanes * 8)
-      asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint8_t*>(p.weight) +
-                                                    static_cast<int64_t>(c0) * wsize));
+  if constexpr (kNorm) {
+    // the weights towards L1, where all rows of the SM read them: a thread a line
+    // (one request a chunk and row group swamped the slices that hold them:
+    // 16384 x 128 10.0 us)
+    const int bytes = p.cols * (p.weight_f32 ? 4 : kSize);
+    for (int b = threadIdx.x * 128; b < bytes; b += blockDim.x * 128)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint8_t*>(p.weight) + b));
   }
   int stage = 0, parity = 0;
   // the same number of turns for every group of a CTA (a CTA has several only
-  // when each is a warp, whose reduction needs no barrier)
+  // when each is a warp or less, whose reduction needs no barrier)
   for (uint32_t base = blockIdx.x * groups; base < rows; base += step) {
     const uint32_t row = base + group;
     const bool live = row < rows;
@@ -585,7 +598,23 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
     }
     reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
     parity ^= 1;
-    if (live && !past_range<kNorm>(sum, most)) {
+    // once more, scaled: a warp with several rows goes together
+    const bool again = live && past_range<kNorm>(sum, most);
+    if (kNorm && (lanes < 32 ? __any_sync(0xffffffffu, again) : again)) {
+      float sum2 = 0.0f, big2 = 0.0f;
+      uint32_t most2;
+#pragma unroll 1
+      for (int c0 = t * 8; again && c0 < cols; c0 += lanes * 8) {
+        float u[8];
+        values(chunk(c0, std::false_type{}), c0, std::true_type{}, u, sum2);
+        big2 = largest(big2, u);
+      }
+      reduce_row<kNorm>(lanes, sum2, big2, most2, s_sum[parity], s_max[parity]);
+      parity ^= 1;
+      if (again)
+        quantize(std::true_type{}, finish_row<kNorm, kE4M3>(p, row, sum2, most2, true, t == 0));
+    }
+    if (live && !again) {
       const float f = finish_row<kNorm, kE4M3>(p, row, sum, most, false, t == 0);
       if (!kHeld || f == 0.0f) {
         quantize(std::false_type{}, f);
@@ -596,16 +625,6 @@ __global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_stag
           if (c0 < cols) put(c0, held[kHeld ? c : 0], f);
         }
       }
-    } else if (live) {  // the same for all threads of the row
-      sum = big = 0.0f;
-#pragma unroll 1
-      for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
-        values(chunk(c0, std::false_type{}), c0, std::true_type{}, held[0], sum);
-        big = largest(big, held[0]);
-      }
-      reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
-      parity ^= 1;
-      quantize(std::true_type{}, finish_row<kNorm, kE4M3>(p, row, sum, most, true, t == 0));
     }
     if constexpr (!kWhole) group_sync(lanes);  // the slot has been read by all
     stage = stage + 1 == p.stages ? 0 : stage + 1;
@@ -813,16 +832,17 @@ cudaError_t launch_mode(const RowsParams& p, bool norm, bool whole, bool staged,
                                : launch_staged<T, kNormed, kE4M3>(p, whole, grid, threads, smem, s);
 }
 
-// Threads per row: four chunks of eight columns each, up to kMaxLanes; a function
-// of the row's length alone (it fixes the order of the sum). With two chunks the
-// per-row work of twice as many warps costs more than it hides (8192 x 4096
-// codes 28.8 us, LANES4). Rows of up to 1024 columns are a warp's, several to a
-// CTA. Rows in flight: two, four of a warp's rows (short ones); the grid is what
-// fits the SMs at once.
+// Threads per row: four chunks of eight columns each, from 4 up to kMaxLanes; a
+// function of the row's length alone (it fixes the order of the sum). With two
+// chunks the per-row work of twice as many warps costs more than it hides (8192
+// x 4096 codes 28.8 us, with four 15.7). Rows of up to 1024 columns are a
+// warp's or a part of it, several to a CTA (a warp each: 100000 x 128 22.4 us).
+// Rows in flight: two, four of such short ones; the grid is what fits the SMs at
+// once.
 template <typename T>
 cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
   constexpr int kSize = sizeof(T);
-  p.lanes = 32;
+  p.lanes = 4;
   while (p.lanes < kMaxLanes && p.lanes * 32 < p.cols) p.lanes *= 2;
   p.inv_cols = 1.0f / static_cast<float>(p.cols);
   const bool residual = norm && p.residual != nullptr;
@@ -834,13 +854,13 @@ cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
                       (!residual || (whole(p.residual, p.ldr) && whole(p.h, p.ldh))) &&
                       (!norm || aligned16(p.weight));
 
-  const int threads = p.lanes == 32 ? 128 : p.lanes;
+  const int threads = p.lanes <= 32 ? 128 : p.lanes;
   const int groups = threads / p.lanes;
   // a chunk past an unaligned row's last block is read (and discarded)
   const int64_t cols8 = static_cast<int64_t>(p.cols + 7) / 8 * 8;
   const int64_t slot = cols8 * kSize + (chunks ? 0 : 32);
   const int64_t streams = residual ? 2 : 1;
-  p.stages = p.lanes == 32 ? 4 : 2;
+  p.stages = p.lanes <= 32 ? 4 : 2;
   if (chunks && p.cols <= kHold * 8 * kMaxLanes && p.lanes > 32 &&
       (slot * streams * 2 + 1536) * (kCtaThreads / threads) > 228 * 1024)
     p.stages = 1;  // as many CTAs as the registers allow before a second row in flight
