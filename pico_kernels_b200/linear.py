@@ -183,6 +183,17 @@ class W8A8Linear(nn.Module):
             layer.bias.copy_(linear.bias.detach().float())
         return layer
 
+    def _apply(self, fn, recurse: bool = True):
+        # Module.to(dtype), half() and the like move the layer and leave its types:
+        # a cast would lose the scales and, e4m3 being a floating type, the codes.
+        before = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, old in before.items():
+            new = self._buffers[name]
+            if old is not None and new.dtype != old.dtype:
+                self._buffers[name] = old.to(new.device)
+        return self
+
     @property
     def weight8(self) -> torch.Tensor:
         """The codes ``[out, in]`` (a view of their padded storage)."""
