@@ -272,3 +272,29 @@ def test_captured_and_replayed_on_another_stream():
     torch.cuda.synchronize()
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("cols", [20, 100, 200, 256, 400, 512])
+def test_rows_that_share_a_warp(cols, code):
+    """Rows of up to 512 columns share a warp: large ones, which the norm goes over
+    twice, and one with a NaN leave their neighbours' bits alone."""
+    x = _x(37, cols, torch.float32, seed=cols)
+    x = x / x.abs().amax(-1, keepdim=True)
+    x[::3] *= 2.0 ** 100
+    x[5, cols // 3] = float("nan")
+    r = x * 0.25
+    w = 1 + 0.3 * torch.randn(cols, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    q, s = pk.rms_norm_quant(x, w, 1e-5, dtype=code)
+    qr, sr, h = pk.rms_norm_quant(x, w, 1e-5, residual=r, dtype=code)
+    good = [i for i in range(37) if i != 5]
+    assert torch.equal(h[good], (x + r)[good])
+    for y, a, b in ((x, q, s), (h, qr, sr)):
+        assert torch.isnan(b[5]) and a.float()[5].abs().max() == 0
+        _check_codes(a[good], b[good], _norm64(y[good], w, 1e-5), 8, (80 / 2 + 8) * U)
+    for i in (0, 4, 6, 7, 36):
+        a, b = pk.rms_norm_quant(x[i:i + 1].clone(), w, 1e-5, dtype=code)
+        assert torch.equal(a.view(torch.uint8)[0], q.view(torch.uint8)[i]) and b[0] == s[i]
+    q, s = pk.quantize_rows(x, code)
+    assert torch.isnan(s[5]) and q.float()[5].abs().max() == 0
+    _check_codes(q[good], s[good], x[good].double(), 3, U)
