@@ -381,7 +381,9 @@ PK_API int pk_gemm_splitk(const void* a, const void* b, int dtype, int64_t M, in
 /* Per-row symmetric quantization of x[M, K] (dtype F16/BF16/F32, ld ldx):
  *   a = max(max_k |x[m, k]|, 1e-12),  scale[m] = a / most,
  *   q[m, k] = round_half_even(x[m, k] * (most / a)),  most = 127 (I8), 448 (E4M3)
- * in fp32. A row with a NaN or an infinity gets scale NaN and codes 0. K < 2^30. */
+ * in fp32 (most / a to a few last places: a product that lies within 2^-21 of its
+ * size from a midpoint may round either way). A row with a NaN or an infinity gets
+ * scale NaN and codes 0. K < 2^30. */
 PK_API int pk_quantize_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
                             int q_dtype, int64_t ldq, float* scale, void* stream);
 
@@ -406,8 +408,8 @@ PK_API int pk_rms_norm_quant(const void* x, int dtype, int64_t M, int64_t K, int
 
 /* out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n] + bias[n]
  * (bias: fp32 [N] or NULL). a and w both I8 (summed exactly in int32; K <=
- * 131071) or both E4M3 (fp32 sums); the scales multiply in fp32 in the order
- * written; out F32, BF16 or F16 (ld ldo). a and w are 16-byte aligned with lda
+ * 131071) or both E4M3 (fp32 sums; K <= 2^24); the scales multiply in fp32 in
+ * the order written; out F32, BF16 or F16 (ld ldo). a and w are 16-byte aligned with lda
  * and ldw multiples of 16 (K itself is free; what lies between K and ld is not
  * read). */
 PK_API int pk_w8a8_gemm(const void* a, int ab_dtype, int64_t lda, const float* a_scale,

@@ -716,6 +716,8 @@ bool at_element(const void* p, int dtype) {
 
 // int32 holds K products of magnitude up to 2^14
 constexpr int64_t kMaxInt8K = (1ll << 17) - 1;
+// a CTA's whole sum has to end well inside the kernels' wait limit
+constexpr int64_t kMaxE4m3K = 1ll << 24;
 
 int run_w8a8(W8A8Args& g, int dtype, cudaStream_t s) {
   const int weights = g.gated ? 2 : 1;
@@ -732,6 +734,9 @@ int run_w8a8(W8A8Args& g, int dtype, cudaStream_t s) {
   if (dtype == PK_I8 && g.K > kMaxInt8K)
     return fail(PK_ERR_SHAPE, "int8 sums are exact for K <= %lld (got %lld)",
                 static_cast<long long>(kMaxInt8K), static_cast<long long>(g.K));
+  if (dtype == PK_E4M3 && g.K > kMaxE4m3K)
+    return fail(PK_ERR_SHAPE, "e4m3 products take K <= %lld (got %lld)",
+                static_cast<long long>(kMaxE4m3K), static_cast<long long>(g.K));
   if (g.lda < g.K || g.ldo < g.N) return fail(PK_ERR_SHAPE, "leading dimension too small");
   if ((reinterpret_cast<uintptr_t>(g.a) & 15) || g.lda % 16 != 0)
     return fail(PK_ERR_ALIGN, "A must be 16-byte aligned with a leading dimension of 16 k");

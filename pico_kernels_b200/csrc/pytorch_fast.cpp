@@ -1,8 +1,9 @@
 // Torch-aware fast-call entry points (module pico_kernels_b200._pktorch).
 //
 // gemm_int4.int4_gemm and int4_gemm_host (and the W8A8 calls of gemm_w8a8 and
-// norm) check a dozen tensor attributes before their C-ABI call; on a slow host CPU each attribute read from Python
-// costs 0.1-0.3 us, together more than the decode GEMM's kernel. These
+// norm) check a dozen tensor attributes before their C-ABI call; on a slow host
+// CPU each attribute read from Python costs 0.1-0.3 us, together more than the
+// decode GEMM's kernel. These
 // functions make the same checks on the tensors in C++ and call
 // libpico_b200.so directly (linked by its soname, so the library instance is
 // the one ctypes loaded). Each returns the output tensor, or the C ABI's

@@ -9,13 +9,15 @@
 //
 // Two kernels:
 //  * w8a8_swap_kernel, few tokens: the weights are the MMA's 128-row operand,
-//    the tokens its 16..256 columns (just as many as needed), one tile per CTA. The product is a weight
-//    stream there; K is split over a thread-block cluster when there are too
-//    few column tiles to keep every SM loading, and the partial sums meet in
-//    distributed shared memory (in rank order; no workspace, no atomics).
+//    the tokens its 16..256 columns (just as many as needed), one tile per CTA.
+//    The product is a weight stream there (16 x 28672 x 8192: 38 us = 6.2 TB/s);
+//    K is split over a thread-block cluster when there are too few column tiles
+//    to keep every SM loading, and the partial sums meet in distributed shared
+//    memory (in rank order; no workspace, no atomics).
 //  * w8a8_pair_kernel, many tokens: persistent, 256 x 256 tiles of a CTA pair
 //    (cta_group::2), two accumulators so that a tile's epilogue overlaps the
-//    next one's main loop. Gated: CTA 0 stages 128 gate channels and CTA 1 the
+//    next one's main loop (4096 x 11008 x 4096 int8: 117 us = 3.2 POP/s, the
+//    tensor cores' rate; held for seconds the power cap makes it 141). Gated: CTA 0 stages 128 gate channels and CTA 1 the
 //    same 128 up channels, so one MMA makes both halves and a row's epilogue
 //    thread holds gate and up of each of its 128 outputs.
 #include <algorithm>
@@ -386,7 +388,8 @@ __global__ void __launch_bounds__(kThreads)
       __syncwarp();
       cluster_sync();
     }
-    const uint32_t red = smem_u32(p.own_red ? smem + stages * stage_bytes + kMaxTokens * 4 + kSwapBars : smem);
+    const uint32_t red = smem_u32(
+        p.own_red ? smem + stages * stage_bytes + kMaxTokens * 4 + kSwapBars : smem);
     if (epi && !fail) {
 #pragma unroll 1
       for (int c = part * (nt / 2); c < (part + 1) * (nt / 2) && c < tokens; c += 8) {
@@ -722,8 +725,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           // Rows off 16-byte boundaries: sixteen columns at a time through
-          // shared memory, so that a warp stores two rows' runs at once (single
-          // stores of 32 rows took 52 us for 333 x 1111 x 1001, DIRECT).
+          // shared memory, so that a warp stores two rows' runs at once (333 x
+          // 1111 x 1001: 16 us, with single stores of 32 rows 52).
 #pragma unroll
           for (int g = 0; g < 32; g += 16) {
 #pragma unroll
@@ -916,8 +919,8 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
 //  * a grid runs in rounds of the CTAs that are resident at once: at one CTA an
 //    SM 148, of clusters of 4 132, of clusters of 8 120;
 //  * swap: 2.5 us of launch and first loads, 0.7 more where a CTA takes most of an
-//    SM's memory (the next kernel's CTAs then wait for it); per token of a tile 13 ns of epilogue
-//    (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
+//    SM's memory (the next kernel's CTAs then wait for it); per token of a tile
+//    13 ns of epilogue (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
 //  * pair: 6 us around the main loop, 0.28 us a K tile (0.21 of a half unit, 0.155
 //    of a quarter).
 constexpr float kSmBytes = 150e3f, kHbmBytes = 6.3e6f, kLatency = 1.6f;  // per us; us
@@ -964,7 +967,8 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
                              : 0.4f + w * nt * (0.030f + 0.020f / split);
   // two CTAs on an SM: a fifth of an epilogue hides behind the other's
   const int64_t full = ctas / (one * occ), rest = ctas % (one * occ);
-  float us = (c.bytes > kMaxSmem / 2 ? 3.2f : 2.5f) + static_cast<float>(full) * (round(one * occ) + epilogue * (occ == 2 ? 1.8f : 1.0f));
+  float us = (c.bytes > kMaxSmem / 2 ? 3.2f : 2.5f) +
+             static_cast<float>(full) * (round(one * occ) + epilogue * (occ == 2 ? 1.8f : 1.0f));
   if (rest > 0) us += round(rest) + epilogue * (rest > one ? 1.8f : 1.0f);
   return us;
 }

@@ -84,7 +84,8 @@ def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.int8
 
     ``scale = max|row|.clamp_min(1e-12) / most`` and ``codes = round(row *
     (most / max|row|))`` in fp32, ``most`` = 127 for int8 (rounded half to
-    even) and 448 for ``float8_e4m3fn``. Returns ``(codes[..., K], scale[...]
+    even; a product that lies within 2^-21 of its size from a midpoint may round
+    either way) and 448 for ``float8_e4m3fn``. Returns ``(codes[..., K], scale[...]
     fp32)`` with ``x ~= codes * scale``. A row that holds a NaN or an infinity
     gets scale NaN and codes 0: its products are NaN, other rows' are not.
     """
@@ -185,7 +186,7 @@ def w8a8_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale
     """``(a8[M, K] @ w8[N, K]^T) * a_scale[m] * w_scale[n] (+ bias[n])``.
 
     ``a8`` and ``w8``: both int8 (summed exactly in int32; K <= 131071) or both
-    ``float8_e4m3fn`` (fp32 sums), as ``quantize_rows`` returns them;
+    ``float8_e4m3fn`` (fp32 sums; K <= 2^24), as ``quantize_rows`` returns them;
     ``a_scale[M]``, ``w_scale[N]`` and ``bias[N]`` fp32. The scales and the
     bias are applied in fp32 in the epilogue and the result rounded once to
     ``out_dtype`` (fp32, bf16 or fp16), into ``out`` when given (a contiguous

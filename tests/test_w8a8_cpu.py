@@ -197,3 +197,35 @@ def test_modules_refuse():
                                                   dtype=torch.bfloat16))]:
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_c_abi_refuses_long_e4m3_sums(gated):
+    lib = _lib.load()
+    K = (1 << 24) + 16
+    if gated:
+        st = lib.pk_w8a8_gated_gemm(64, E4, K, 64, 64, K, 64, 64, K, 64, 0, 1, 1, K, 64, F32, 1, None)
+    else:
+        st = lib.pk_w8a8_gemm(64, E4, K, 64, 64, K, 64, None, 1, 1, K, 64, F32, 1, None)
+    assert st == _lib.PK_ERR_SHAPE
+
+
+@pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])
+def test_linear_keeps_its_types(code):
+    """Casts of a module tree move the layer but change neither codes nor scales."""
+    layer = pk.W8A8Linear(20, 6, dtype=code)
+    layer.codes.view(torch.uint8).random_(0, 120)
+    layer.scales.uniform_()
+    layer.bias.uniform_()
+    codes, scales, bias = (t.clone() for t in (layer.codes, layer.scales, layer.bias))
+    tree = torch.nn.Sequential(torch.nn.Linear(4, 4), layer)
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(),
+                 lambda m: m.to("cpu", torch.float16)):
+        cast(tree)
+        assert tree[0].weight.dtype != torch.float32
+        assert layer.codes.dtype == code
+        assert torch.equal(layer.codes.view(torch.uint8), codes.view(torch.uint8))
+        assert torch.equal(layer.scales, scales) and torch.equal(layer.bias, bias)
+    loaded = pk.W8A8Linear(20, 6, dtype=code).half()
+    loaded.load_state_dict(layer.state_dict())
+    assert torch.equal(loaded.scales, scales)
