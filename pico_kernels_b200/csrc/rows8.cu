@@ -9,8 +9,8 @@
 //
 // All three are bound by HBM: a row is read once, kept while its sum and its
 // largest magnitude are reduced, and written once (4096 x 28672 bf16 to int8
-// 55 us = 6.4 TB/s; the norm of 4096 x 8192 with a residual 41 us = 5.7 TB/s,
-// without one 25 us = 4.0 TB/s, where 16 instructions a value and the
+// 55 us = 6.4 TB/s; the norm of 4096 x 8192 with a residual 40 us = 5.9 TB/s,
+// without one 22.5 us = 4.5 TB/s, where 16 instructions a value and the
 // reduction's round trip between a row's passes take longer than its bytes).
 // The norm needs one reduction, not two (the sum for r, then the maximum of y): r multiplies
 // the whole row, so the codes of y are those of u_k = h_k * w_k, and the sum of
@@ -419,7 +419,16 @@ enum Mode : int { kCodes = 0, kNormed = 1, kSummed = 2 };
 
 constexpr int kHold = 4;  // chunks of a row a thread holds as fp32
 
-constexpr int kCtaThreads = 1024;  // threads an SM holds of it: 64 registers each
+// Threads an SM holds of a kernel, hence the registers of one. The norm of whole
+// rows spills at 64 registers and is faster with fewer threads of 80 (4096 x 8192
+// 25.4 -> 22.5 us, 4096 x 5120 with a residual 28.3 -> 24.6; 16384 columns, one CTA
+// an SM, 25.1 -> 26.0); the quantizer, whose long rows live from what is in flight,
+// and the norm of other rows are not (codes 4096 x 28672 55 -> 62 us, norm 1000 x
+// 5001 9.3 -> 9.9).
+constexpr int sm_threads(Mode mode, bool whole, bool held) {
+  return mode != kCodes && whole && held ? 768 : 1024;
+}
+constexpr int thread_regs(int threads) { return 65536 / threads / 8 * 8; }
 
 // Rows staged in shared memory. A group of `lanes` threads walks its rows with
 // `stages` of them in flight (cp.async): a thread copies the chunks it will
@@ -436,7 +445,8 @@ constexpr int kCtaThreads = 1024;  // threads an SM holds of it: 64 registers ea
 // 23 (codes) to 46 (norm with a residual) of them and the SMs issued at 70 % of
 // their rate (4096 x 8192 with a residual 54.9 us).
 template <typename T, Mode kMode, bool kE4M3, bool kWhole, bool kHeld>
-__global__ void __launch_bounds__(kMaxLanes, kCtaThreads / kMaxLanes) rows8_staged_kernel(const RowsParams p) {
+__global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
+    rows8_staged_kernel(const RowsParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_sum[2][32];
   __shared__ uint32_t s_max[2][32];
@@ -867,8 +877,10 @@ cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
   const int64_t slot = cols8 * kSize + (chunks ? 0 : 32);
   const int64_t streams = residual ? 2 : 1;
   p.stages = p.lanes <= 32 ? 4 : 2;
-  if (chunks && p.cols <= kHold * 8 * kMaxLanes && p.lanes > 32 &&
-      (slot * streams * 2 + 1536) * (kCtaThreads / threads) > 228 * 1024)
+  const bool held = !chunks || p.cols <= kHold * 8 * kMaxLanes;
+  const int resident =
+      sm_threads(!norm ? kCodes : residual ? kSummed : kNormed, chunks, held) / threads;
+  if (chunks && held && p.lanes > 32 && (slot * streams * 2 + 1536) * resident > 228 * 1024)
     p.stages = 1;  // as many CTAs as the registers allow before a second row in flight
   const int64_t bytes = slot * streams * groups * p.stages;
   const int64_t widest = std::max({p.ldx, p.ldr, p.ldh, p.ldq}) * kSize;
@@ -879,8 +891,8 @@ cudaError_t launch_rows(RowsParams p, bool norm, cudaStream_t s) {
   const bool staged = bytes <= kMostStaged && widest < (1ll << 32) &&
                       (chunks || p.cols <= kHold * 8 * kMaxLanes);
   p.slot = static_cast<int>(staged ? slot : 0);
-  const int64_t per_sm = std::max<int64_t>(
-      1, std::min<int64_t>(kCtaThreads / threads, 228 * 1024 / (bytes + 1536)));
+  const int64_t per_sm =
+      std::max<int64_t>(1, std::min<int64_t>(resident, 228 * 1024 / (bytes + 1536)));
   const int64_t ctas = (p.rows + groups - 1) / groups;
   const int grid =
       static_cast<int>(staged ? std::min<int64_t>(ctas, per_sm * num_sms()) : p.rows);
