@@ -298,3 +298,23 @@ def test_rows_that_share_a_warp(cols, code):
     q, s = pk.quantize_rows(x, code)
     assert torch.isnan(s[5]) and q.float()[5].abs().max() == 0
     _check_codes(q[good], s[good], x[good].double(), 3, U)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cols", [2, 9, 33, 250, 255, 1001, 1003, 2047, 5001])
+def test_residual_streams_of_odd_width(cols, dt):
+    """Rows off 16-byte boundaries: h is stored in blocks that span two threads'
+    chunks, in place as well, and in a tensor that starts at any element."""
+    x, r = _x(67, cols, dt, seed=cols), _x(67, cols, dt, seed=cols + 1)
+    w = torch.ones(cols, device="cuda")
+    want = (x.float() + r.float()).to(dt)
+    q, s, h = pk.rms_norm_quant(x, w, residual=r)
+    assert torch.equal(h, want)
+    for shift in (0, 1, 3):
+        flat = torch.full((67 * cols + 8,), 5.0, device="cuda", dtype=dt)
+        out = flat[shift:shift + 67 * cols].view(67, cols)
+        out.copy_(r)
+        q2, s2, h2 = pk.rms_norm_quant(x, w, residual=out, residual_out=out)
+        assert h2.data_ptr() == out.data_ptr() and torch.equal(out, want)
+        assert (flat[:shift] == 5).all() and (flat[shift + 67 * cols:] == 5).all()
+        assert torch.equal(q, q2) and torch.equal(s, s2)
