@@ -789,13 +789,14 @@ Params params_of(const W8A8Args& g) {
   return p;
 }
 
-constexpr int kMaxSmem = 226 * 1024;
+constexpr int kMaxSmem = 226 * 1024;  // for a ring and what follows it
+constexpr int kAllSmem = 227 * 1024;
 
 template <typename Kernel>
 cudaError_t launch(Kernel kernel, int grid, int threads, int cluster, int smem, cudaStream_t s,
                    const CUtensorMap (&tm)[3], const Params& p) {
   // the attribute once and for all sizes (a plan's size changes from call to call)
-  cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), kMaxSmem);
+  cudaError_t e = set_max_smem(reinterpret_cast<const void*>(kernel), kAllSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attrs[2];
@@ -824,7 +825,7 @@ struct Plan {
 
 // Shared memory of a swap CTA: its ring, and what follows it.
 struct SwapSmem {
-  int stages, stage_bytes, own_red, bytes;
+  int stages, stage_bytes, own_red, bytes, tmem_cols;
   bool fits;
 };
 
@@ -844,6 +845,16 @@ SwapSmem swap_smem(const Plan& plan, bool gated, int64_t k_tiles) {
     while (c.stages * c.stage_bytes < sums && (c.stages + 1) * c.stage_bytes <= whole) ++c.stages;
   c.fits = sums == 0 || c.own_red || sums <= c.stages * c.stage_bytes;
   c.bytes = c.stages * c.stage_bytes + rest;
+  c.tmem_cols = 32;
+  while (c.tmem_cols < plan.nt * w * plan.pieces) c.tmem_cols *= 2;
+  // CTAs of a cluster wait for one another with their tensor memory held. Two
+  // clusters of different streams that share two SMs must therefore never ask
+  // for more of it than there is, or each may hold on one SM what the other
+  // waits for on the other: a CTA of a split takes at least the share of the
+  // SM's 228 KB (1 KB a CTA is the system's) that its columns are of the 512,
+  // and no less than 40 KB, which leaves it no room beside a kernel that takes
+  // all 512 columns with 194 KB of its own.
+  if (plan.split > 1) c.bytes = std::max({c.bytes, c.tmem_cols * (228 * 1024 / 512) - 1024, 40 * 1024});
   return c;
 }
 
@@ -868,8 +879,7 @@ cudaError_t launch_swap(const W8A8Args& g, const Plan& plan, cudaStream_t s, con
   p.stage_bytes = c.stage_bytes;
   p.own_red = c.own_red;
   p.pieces = plan.pieces;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < plan.nt * (kGated ? 2 : 1) * plan.pieces) p.tmem_cols *= 2;
+  p.tmem_cols = c.tmem_cols;
   p.num_m = static_cast<int>(ceil_div(g.M, plan.nt));
   p.num_n = static_cast<int>(ceil_div(g.N, 128));
   const int64_t grid = static_cast<int64_t>(p.num_m) * p.num_n * p.split;

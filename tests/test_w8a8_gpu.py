@@ -353,3 +353,34 @@ def test_block_captured_twice_and_replayed_at_once():
     torch.cuda.synchronize()
     for o, want_o in zip(outs, want):
         assert all(torch.equal(a, b) for a, b in zip(o, want_o))
+
+
+def test_products_of_several_streams_at_once():
+    """Clusters of different sizes share SMs and their tensor memory: the results
+    are those of the calls one after another."""
+    sizes = [(1, 512, 4096), (16, 256, 16384), (40, 384, 8192), (130, 640, 4096), (200, 512, 4096),
+             (256, 256, 8192), (300, 1024, 512)]
+    calls = []
+    for i, (M, N, K) in enumerate(sizes):
+        for code in CODES:
+            g = torch.Generator(device="cuda").manual_seed(i)
+            a, w, u = (_codes(r, K, code, g) for r in (M, N, N))
+            sa, sw, su = (torch.rand(r, device="cuda", generator=g) for r in (M, N, N))
+            calls.append(lambda a=a, sa=sa, w=w, sw=sw: pk.w8a8_gemm(a, sa, w, sw))
+            calls.append(lambda a=a, sa=sa, w=w, sw=sw, u=u, su=su:
+                         pk.w8a8_gated_gemm(a, sa, w, sw, u, su, out_dtype=torch.float16))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(4):
+        got = [[] for _ in streams]
+        for j in range(len(calls)):
+            for s, stream in enumerate(streams):
+                k = (j * (2 * s + 1) + 5 * s + turn) % len(calls)
+                with torch.cuda.stream(stream):
+                    got[s].append((k, calls[k]()))
+        torch.cuda.synchronize()
+        for rows in got:
+            for k, y in rows:
+                assert torch.equal(y.nan_to_num(), want[k].nan_to_num()), sizes[k // 4]
+    assert pk.device_status()[0] == 0
