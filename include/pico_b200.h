@@ -380,10 +380,11 @@ PK_API int pk_gemm_splitk(const void* a, const void* b, int dtype, int64_t M, in
 
 /* Per-row symmetric quantization of x[M, K] (dtype F16/BF16/F32, ld ldx):
  *   a = max(max_k |x[m, k]|, 1e-12),  scale[m] = a / most,
- *   q[m, k] = round_half_even(x[m, k] * (most / a)),  most = 127 (I8), 448 (E4M3)
- * in fp32 (most / a to a few last places: a product that lies within 2^-21 of its
- * size from a midpoint may round either way). A row with a NaN or an infinity gets
- * scale NaN and codes 0. K < 2^30. */
+ *   q[m, k] = round_half_even(x[m, k] * most / a),  most = 127 (I8), 448 (E4M3)
+ * where the quotient is rounded to fp32 before it goes to the nearest code: of 16-bit
+ * x every code is the nearest, half steps to even; of fp32 x a quotient within
+ * 2^-24 of its size from a midpoint may take either side. A row with a NaN or an
+ * infinity gets scale NaN and codes 0. K < 2^30. */
 PK_API int pk_quantize_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
                             int q_dtype, int64_t ldq, float* scale, void* stream);
 

@@ -2,15 +2,15 @@
 // row, its inverse, and the RMS norm that writes its output already quantized.
 //
 //   quantize      a = max(max_k |x_k|, 1e-12),  scale = a / most,
-//                 q_k = round(x_k * (most / a)),  most = 127 (int8) or 448 (e4m3)
+//                 q_k = round(x_k * most / a),  most = 127 (int8) or 448 (e4m3)
 //   rms norm      h = T(x + residual),  r = 1 / sqrt(mean(h^2) + eps),
 //                 y_k = h_k * r * w_k, quantized as above
 //   dequantize    x_k = q_k * scale
 //
 // All three are bound by HBM: a row is read once, kept while its sum and its
-// largest magnitude are reduced, and written once (4096 x 28672 bf16 to int8
-// 55 us = 6.4 TB/s; the norm of 4096 x 8192 with a residual 40 us = 5.9 TB/s,
-// without one 22.5 us = 4.5 TB/s, where 16 instructions a value and the
+// largest magnitude are reduced, and written once (4096 x 28672 bf16 to e4m3
+// 57 us = 6.1 TB/s; the norm of 4096 x 8192 with a residual 40 us = 5.9 TB/s,
+// without one 23.6 us = 4.3 TB/s, where about 16 instructions a value and the
 // reduction's round trip between a row's passes take longer than its bytes).
 // The norm needs one reduction, not two (the sum for r, then the maximum of y): r multiplies
 // the whole row, so the codes of y are those of u_k = h_k * w_k, and the sum of
@@ -22,7 +22,9 @@
 // and codes 0, so that every product with it is NaN and no other row is
 // touched. Sums, maxima and scales are fp32; the only roundings to fewer bits
 // are the stored h (the residual stream's own type, which is what the next
-// layer adds to, so the norm is that of the stored value) and the codes.
+// layer adds to, so the norm is that of the stored value) and the codes, which are
+// the nearest to quotients that carry one fp32 rounding: a half step is met as
+// such, and goes to even.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -292,17 +294,47 @@ __device__ __forceinline__ void store_shifted8(T* row, int c0, int cols, const E
   }
 }
 
-// Four int8 codes of u * f: adding 1.5 * 2^23 leaves the product, rounded half
-// to even by the addition (fused: one rounding), as an integer in the low bits.
-// |u * f| is at most 127 and a few last places, so no code passes 127. One
-// multiply-add a value and three byte selections, where conversions, clamps and
-// shifts took eight instructions.
-__device__ __forceinline__ uint32_t int8_codes4(const float* u, float f) {
+// What takes a row's u to its codes: most / max|u| as the sum of two fp32 numbers
+// (both 0: the row has no 8-bit form).
+struct Factor {
+  float hi, lo;
+};
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
+// Two quotients u * most / max|u|, each rounded to fp32 once (off by 2^-24 of
+// itself): with the factor as one fp32 number a quotient that is a half step of
+// the codes came out beside it, and values of 16 bits hit half steps often. It
+// costs a packed multiplication per two values, and int8 a packed addition (codes
+// 4096 x 28672 55.2 -> 57.3 us, 4096 x 11008 22.1 -> 23.8; the norm of 4096 x 8192
+// 22.5 -> 23.6, with a residual nothing).
+__device__ __forceinline__ uint64_t quotients2(float a, float b, Factor f) {
+  const uint64_t u = pack2(a, b);
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(u), "l"(pack2(f.lo, f.lo)));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(r) : "l"(u), "l"(pack2(f.hi, f.hi)));
+  return r;
+}
+
+// Four int8 codes: adding 1.5 * 2^23 leaves the quotient, rounded half to even by
+// the addition, as an integer in the low bits. A quotient is at most 127 and a
+// last place, so no code passes 127.
+__device__ __forceinline__ uint32_t int8_codes4(const float* u, Factor f) {
   constexpr float kMagic = 12582912.0f;
-  uint32_t b[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(fmaf(u[j], f, kMagic));
-  return prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
+  uint64_t a = quotients2(u[0], u[1], f), b = quotients2(u[2], u[3], f);
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(pack2(kMagic, kMagic)));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(b) : "l"(pack2(kMagic, kMagic)));
+  return prmt(prmt(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040),
+              prmt(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), 0x0040), 0x5410);
 }
 
 // Largest of |a|, |b|, |c|; NaN if one is NaN.
@@ -313,12 +345,12 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 }
 
 template <bool kE4M3>
-__device__ __forceinline__ uint32_t codes4(const float* u, float f) {
+__device__ __forceinline__ uint32_t codes4(const float* u, Factor f) {
   if constexpr (kE4M3) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(u[0] * f, u[1] * f), __NV_SATFINITE,
-                                                 __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(u[2] * f, u[3] * f), __NV_SATFINITE,
-                                                 __NV_E4M3);
+    const uint32_t lo =
+        __nv_cvt_float2_to_fp8x2(unpack2(quotients2(u[0], u[1], f)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi =
+        __nv_cvt_float2_to_fp8x2(unpack2(quotients2(u[2], u[3], f)), __NV_SATFINITE, __NV_E4M3);
     return prmt(lo, hi, 0x5410);
   } else {
     return int8_codes4(u, f);
@@ -329,7 +361,7 @@ __device__ __forceinline__ uint32_t codes4(const float* u, float f) {
 // (kWhole), else as the row's end and the caller's pitch allow.
 template <bool kE4M3, bool kWhole>
 __device__ __forceinline__ void store_codes(uint8_t* q, int c0, int cols, bool vec,
-                                            const float (&u)[8], float f) {
+                                            const float (&u)[8], Factor f) {
   const uint32_t lo = codes4<kE4M3>(u, f), hi = codes4<kE4M3>(u + 4, f);
   if (kWhole || (vec && c0 + 8 <= cols)) {
     *reinterpret_cast<uint2*>(q + c0) = make_uint2(lo, hi);
@@ -378,23 +410,29 @@ __device__ __forceinline__ void reduce_row(int lanes, float& sum, float big, uin
   if constexpr (kNorm) sum = warp_sum(lane < warps ? s_sum[lane] : 0.0f);
 }
 
-// A row from its reductions: its scale (stored by one thread) and the factor
-// that takes u to codes; 0 for a row that has no 8-bit form.
+// A row from its reductions: its scale (stored by one thread) and its factor. In
+// most / a the norm's r cancels, unless the row's maximum is the least there is.
 constexpr float kDown = 8.271806125530277e-25f;  // 2^-80
 template <bool kNorm, bool kE4M3>
-__device__ __forceinline__ float finish_row(const RowsParams& p, int64_t row, float sum,
+__device__ __forceinline__ Factor finish_row(const RowsParams& p, int64_t row, float sum,
                                             uint32_t most, bool scaled, bool store) {
-  // Every warp of the row does this, once a row: reciprocals by the special
-  // function unit (2 last places; __fdividef flushes nothing here, a is normal),
-  // the IEEE division only in the thread that stores the scale. With IEEE
-  // divisions throughout it cost as many instructions as a thread's values.
   constexpr float top = kE4M3 ? 448.0f : 127.0f;
   const float r = kNorm ? rsqrtf(fmaf(sum, p.inv_cols, scaled ? 0.0f : p.eps)) : 1.0f;
-  const float a = fmaxf(__uint_as_float(most) * r, kTiny);
+  const float big = __uint_as_float(most) * r;
+  const float a = fmaxf(big, kTiny);
   const bool bad = most >= kInfBits || !(a < __uint_as_float(kInfBits)) || (kNorm && !(r > 0.0f));
   if (store) p.scale[row] = bad ? __uint_as_float(0x7fc00000u) : a / top;
-  const float f = a < 1e36f ? __fdividef(top, a) : top / a;
-  return bad ? 0.0f : (kNorm ? r * f : f);
+  const bool least = !(big > kTiny);
+  const float by = least ? kTiny : __uint_as_float(most);
+  Factor f;
+  f.hi = top / by;
+  f.lo = fmaf(-f.hi, by, top) * (f.hi * (1.0f / top));  // what is left of top, over by
+  if (kNorm && least) {
+    f.hi *= r;
+    f.lo *= r;
+  }
+  if (bad) f = {0.0f, 0.0f};
+  return f;
 }
 
 // Magnitudes above ~1e19 square past fp32's range, and a product with a weight
@@ -610,14 +648,14 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
       for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
       return big;
     };
-    auto put = [&](int c0, const float (&u)[8], float f) {
+    auto put = [&](int c0, const float (&u)[8], Factor f) {
       store_codes<kE4M3, kWhole>(q, c0, p.cols, p.codes_vec, u, f);
     };
-    auto quantize = [&](auto scaled, float f) {  // from the staged row
+    auto quantize = [&](auto scaled, Factor f) {  // from the staged row
 #pragma unroll 2
       for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
         float u[8] = {}, unused = 0.0f;
-        if (f != 0.0f) values(chunk(c0, std::false_type{}), c0, scaled, u, unused);
+        if (f.hi != 0.0f) values(chunk(c0, std::false_type{}), c0, scaled, u, unused);
         put(c0, u, f);
       }
     };
@@ -670,8 +708,8 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
         quantize(std::true_type{}, finish_row<kNorm, kE4M3>(p, row, sum2, most2, true, t == 0));
     }
     if (live && !again) {
-      const float f = finish_row<kNorm, kE4M3>(p, row, sum, most, false, t == 0);
-      if (!kHeld || f == 0.0f) {
+      const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, false, t == 0);
+      if (!kHeld || f.hi == 0.0f) {
         quantize(std::false_type{}, f);
       } else {
 #pragma unroll
@@ -742,11 +780,11 @@ __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams 
     factor = kDown;
     pass(false, 1);
   }
-  const float f = finish_row<kNorm, kE4M3>(p, row, sum, most, scaled, t == 0);
+  const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, scaled, t == 0);
   for (int c0 = t * 8; c0 < p.cols; c0 += kMaxLanes * 8) {
     float u[8], unused = 0.0f;
     values(false, factor, c0, u, unused);
-    if (f == 0.0f) {
+    if (f.hi == 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = 0.0f;
     }

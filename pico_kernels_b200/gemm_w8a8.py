@@ -83,11 +83,12 @@ def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.int8
     """Quantize ``x[..., K]`` (fp16, bf16 or fp32) to 8 bits, one scale per row.
 
     ``scale = max|row|.clamp_min(1e-12) / most`` and ``codes = round(row *
-    (most / max|row|))`` in fp32, ``most`` = 127 for int8 (rounded half to
-    even; a product that lies within 2^-21 of its size from a midpoint may round
-    either way) and 448 for ``float8_e4m3fn``. Returns ``(codes[..., K], scale[...]
-    fp32)`` with ``x ~= codes * scale``. A row that holds a NaN or an infinity
-    gets scale NaN and codes 0: its products are NaN, other rows' are not.
+    most / max|row|)``, half steps to even, ``most`` = 127 for int8 and 448 for
+    ``float8_e4m3fn``. Codes of 16-bit rows are the nearest there are; of fp32
+    rows a quotient within 2^-24 of its size from a midpoint may take either
+    side. Returns ``(codes[..., K], scale[...] fp32)`` with ``x ~= codes *
+    scale``. A row that holds a NaN or an infinity gets scale NaN and codes 0:
+    its products are NaN, other rows' are not.
     """
     tf = _lib.torch_fast()
     if tf is not None:

@@ -318,3 +318,65 @@ def test_residual_streams_of_odd_width(cols, dt):
         assert h2.data_ptr() == out.data_ptr() and torch.equal(out, want)
         assert (flat[:shift] == 5).all() and (flat[shift + 67 * cols:] == 5).all()
         assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+def _tie_rows(code, dt, cols, g):
+    """Rows with a largest value of 7 k 2^j (e4m3) or 127 2^j (int8), for which a
+    row's half steps are numbers of its type: most / max then has no short form."""
+    rows = []
+    for i in range(24):
+        if code == torch.int8:
+            k, top = 1, 127
+            v = torch.randint(-127, 127, (cols,), device="cuda", generator=g) + 0.5
+        else:
+            k, top = (1, 3, 5, 7)[i % 4], 448
+            m = torch.randint(8, 16, (cols,), device="cuda", generator=g) + 0.5
+            e = torch.randint(-6, 5, (cols,), device="cuda", generator=g)
+            v = m * torch.exp2(e.float()) * (1 - 2 * torch.randint(0, 2, (cols,), device="cuda", generator=g))
+        v = (v * k).clamp(-top * k, top * k)
+        v[i % cols] = top * k
+        rows.append(v * 2.0 ** (i // 4 - 8))
+    x = torch.stack(rows)
+    assert torch.equal(x.to(dt).float(), x)
+    return x.to(dt)
+
+
+def _nearest_codes(u, code):
+    """Rows in 64 bits to their codes: u * most / max|u|, half steps to even."""
+    most = 127.0 if code == torch.int8 else 448.0
+    t = u * most / u.abs().amax(-1, keepdim=True)
+    if code == torch.int8:
+        return t.round()
+    step = torch.exp2(torch.floor(torch.log2(t.abs().clamp_min(2.0 ** -6))) - 3)
+    return (t / step).round() * step
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [1, 9, 100, 1000, 1001, 4096, 16392, 33000])
+def test_codes_of_16_bit_rows_are_the_nearest(cols, dt, code):
+    """Exactly: u and max|u| have at most 11 bits, so a quotient u * most / max|u| that
+    is no half step lies at least 2^-20 of its size away from one, and 64 bits
+    (2^-52) and the kernel's fp32 (2^-24) round it alike; a half step goes to even."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    for x in (_tie_rows(code, dt, cols, g), _x(200, cols, dt, seed=cols)):
+        q = pk.quantize_rows(x, code)[0]
+        assert torch.equal(q.double(), _nearest_codes(x.double(), code))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("cols", [1, 9, 100, 1000, 1001, 4096, 16392, 33000])
+def test_codes_of_bf16_norms_are_the_nearest(cols, residual, code):
+    """r = 1 / sqrt(mean + eps) multiplies the whole row, so the codes are those of
+    h * w, which fp32 holds exactly (16 bits). A quotient that is no half step is
+    off one by at least 1 / (2 * 2^16) of a row maximum of 127 (int8; farther in
+    e4m3), 2^-24 of its size, which fp32 tells apart."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    one = torch.ones(cols, device="cuda", dtype=torch.bfloat16)
+    for x, w in ((_tie_rows(code, torch.bfloat16, cols, g), one),
+                 (_x(200, cols, torch.bfloat16, seed=cols),
+                  (1 + 0.3 * torch.randn(cols, device="cuda", generator=g)).bfloat16())):
+        r = torch.zeros_like(x) if residual else None
+        q = pk.rms_norm_quant(x, w, 1e-5, residual=r, dtype=code)[0]
+        assert torch.equal(q.double(), _nearest_codes(x.double() * w.double(), code))
