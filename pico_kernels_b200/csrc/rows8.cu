@@ -727,13 +727,16 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
 
 // Rows of which the stages do not fit shared memory, rows of more than 16384
 // columns that are not whole 16-byte chunks, and rows 4 GB or more apart: one CTA
-// a row, read again, from L2, for the codes.
+// a row, read again, from L2, for the codes. The row's threads and the order of its
+// sum are those of the staged kernel, whatever its width: a CTA of `lanes` threads,
+// or one warp of which `lanes` hold the row and the rest hold nothing.
 template <typename T, bool kNorm, bool kE4M3>
 __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams p) {
   __shared__ float s_sum[2][32];
   __shared__ uint32_t s_max[2][32];
   const int64_t row = blockIdx.x;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, lanes = p.lanes;
+  const int begin = t < lanes ? t * 8 : p.cols;
   griddep_wait();
   griddep_launch_dependents();
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
@@ -766,22 +769,23 @@ __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams 
   auto pass = [&](bool start, int parity) {
     float big = 0.0f;
     sum = 0.0f;
-    for (int c0 = t * 8; c0 < p.cols; c0 += kMaxLanes * 8) {
+    for (int c0 = begin; c0 < p.cols; c0 += lanes * 8) {
       float u[8];
       values(start, factor, c0, u, sum);
 #pragma unroll
       for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
     }
-    reduce_row<kNorm>(kMaxLanes, sum, big, most, s_sum[parity], s_max[parity]);
+    reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
   };
   pass(true, 0);
-  const bool scaled = past_range<kNorm>(sum, most);
+  bool scaled = past_range<kNorm>(sum, most);
+  if (lanes < 32) scaled = __any_sync(0xffffffffu, scaled);  // the whole warp as the row
   if (scaled) {
     factor = kDown;
     pass(false, 1);
   }
   const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, scaled, t == 0);
-  for (int c0 = t * 8; c0 < p.cols; c0 += kMaxLanes * 8) {
+  for (int c0 = begin; c0 < p.cols; c0 += lanes * 8) {
     float u[8], unused = 0.0f;
     values(false, factor, c0, u, unused);
     if (f.hi == 0.0f) {
@@ -918,9 +922,11 @@ cudaError_t launch_staged(const RowsParams& p, bool whole, dim3 grid, int thread
 template <typename T, bool kE4M3>
 cudaError_t launch_mode(const RowsParams& p, bool norm, bool whole, bool staged, int threads,
                         int grid, int smem, cudaStream_t s) {
-  if (!staged)
-    return norm ? launch_chained(rows8_long_kernel<T, true, kE4M3>, grid, threads, 0, s, p)
-                : launch_chained(rows8_long_kernel<T, false, kE4M3>, grid, threads, 0, s, p);
+  if (!staged) {
+    const int block = std::max(p.lanes, 32);
+    return norm ? launch_chained(rows8_long_kernel<T, true, kE4M3>, grid, block, 0, s, p)
+                : launch_chained(rows8_long_kernel<T, false, kE4M3>, grid, block, 0, s, p);
+  }
   if (!norm) return launch_staged<T, kCodes, kE4M3>(p, whole, grid, threads, smem, s);
   return p.residual != nullptr ? launch_staged<T, kSummed, kE4M3>(p, whole, grid, threads, smem, s)
                                : launch_staged<T, kNormed, kE4M3>(p, whole, grid, threads, smem, s);

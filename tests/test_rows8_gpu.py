@@ -380,3 +380,61 @@ def test_codes_of_bf16_norms_are_the_nearest(cols, residual, code):
         r = torch.zeros_like(x) if residual else None
         q = pk.rms_norm_quant(x, w, 1e-5, residual=r, dtype=code)[0]
         assert torch.equal(q.double(), _nearest_codes(x.double() * w.double(), code))
+
+
+@pytest.fixture(scope="module")
+def far_buffer():
+    yield torch.zeros((1 << 32) + (1 << 18), device="cuda", dtype=torch.uint8)
+
+
+def _far(buf, x):
+    """x's two rows 4 GiB apart."""
+    n = (1 << 32) // x.element_size()
+    y = torch.as_strided(buf.view(x.dtype), x.shape, (n, 1))
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cols", [1, 7, 20, 100, 128, 129, 300, 512, 1000, 1024, 1032, 2047, 4096,
+                                  5001, 8192, 16384, 16385])
+def test_rows_gigabytes_apart(cols, dt, far_buffer):
+    """The bits of the same rows side by side: codes, scales and sums do not depend
+    on strides, whichever kernel a distance needs."""
+    x = _x(2, cols, dt, seed=cols)
+    w = 1 + 0.3 * torch.randn(cols, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    for big in ((1.0, 2.0 ** 80) if dt != torch.float16 else (1.0,)):  # squares in and past fp32
+        x = torch.stack((x[0], (x[1].float() * big).to(dt)))
+        r = (x * 0.5).flip(1)
+        for code in CODES:
+            want = (pk.quantize_rows(x, code), pk.rms_norm_quant(x, w, dtype=code),
+                    pk.rms_norm_quant(x, w, residual=r, dtype=code),
+                    pk.rms_norm_quant(r, w, residual=x, dtype=code))
+            y = _far(far_buffer, x)
+            got = (pk.quantize_rows(y, code), pk.rms_norm_quant(y, w, dtype=code),
+                   pk.rms_norm_quant(y, w, residual=r, dtype=code),
+                   pk.rms_norm_quant(r, w, residual=y, dtype=code))
+            for a, b in zip(want, got):
+                for s, t in zip(a, b):
+                    assert torch.equal(s.float(), t.float())
+            q, s = want[0]
+            assert torch.equal(pk.dequantize_rows(_far(far_buffer, q), s), pk.dequantize_rows(q, s))
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cols", [16376, 16383, 16384, 16385])
+def test_rows_around_the_widest_that_threads_hold(cols, dt, residual):
+    w = 1 + 0.3 * torch.randn(cols, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    for rows, code in ((1, torch.int8), (5, torch.float8_e4m3fn), (300, torch.int8)):
+        x = _x(rows, cols, dt, seed=rows)
+        q, s = pk.quantize_rows(x, code)
+        _check_codes(q, s, x.double(), 3, U)
+        h = x
+        if residual:
+            r = _x(rows, cols, dt, seed=rows + 7)
+            q, s, h = pk.rms_norm_quant(x, w, 1e-5, residual=r, dtype=code)
+            assert torch.equal(h, (x.float() + r.float()).to(dt))
+        else:
+            q, s = pk.rms_norm_quant(x, w, 1e-5, dtype=code)
+        _check_codes(q, s, _norm64(h, w, 1e-5), 8, (80 / 2 + 8) * U)
