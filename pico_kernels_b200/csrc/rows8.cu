@@ -412,12 +412,11 @@ __device__ __forceinline__ void reduce_row(int lanes, float& sum, float big, uin
 
 // A row from its reductions: its scale (stored by one thread) and its factor. In
 // most / a the norm's r cancels, unless the row's maximum is the least there is.
-constexpr float kDown = 8.271806125530277e-25f;  // 2^-80
 template <bool kNorm, bool kE4M3>
 __device__ __forceinline__ Factor finish_row(const RowsParams& p, int64_t row, float sum,
-                                            uint32_t most, bool scaled, bool store) {
+                                            uint32_t most, bool store) {
   constexpr float top = kE4M3 ? 448.0f : 127.0f;
-  const float r = kNorm ? rsqrtf(fmaf(sum, p.inv_cols, scaled ? 0.0f : p.eps)) : 1.0f;
+  const float r = kNorm ? rsqrtf(fmaf(sum, p.inv_cols, p.eps)) : 1.0f;
   const float big = __uint_as_float(most) * r;
   const float a = fmaxf(big, kTiny);
   const bool bad = most >= kInfBits || !(a < __uint_as_float(kInfBits)) || (kNorm && !(r > 0.0f));
@@ -435,13 +434,65 @@ __device__ __forceinline__ Factor finish_row(const RowsParams& p, int64_t row, f
   return f;
 }
 
-// Magnitudes above ~1e19 square past fp32's range, and a product with a weight
-// may pass it: such a row goes over its values once more as h * 2^-80, which
-// cancels in the norm (eps does not reach such sums). A true infinity or NaN
-// stays one.
+// Magnitudes above ~1e19 square past fp32's range, and h * weight may pass it where
+// h * r * weight does not.
 template <bool kNorm>
 __device__ __forceinline__ bool past_range(float sum, uint32_t most) {
   return kNorm && (!(sum < __uint_as_float(kInfBits)) || most >= kInfBits);
+}
+
+// Such a row, from memory: its sum once more, of h * 2^-80 where the squares need it,
+// then the maximum of y = h * r * weight itself, whose codes are made as the
+// quantizer's. A true infinity or NaN stays one. The row's threads come here together
+// (and with them the rows that share their warp, which are not `mine`); what was
+// written of h is visible to them. An even number of reductions: the buffers'
+// turn is the caller's again afterwards. (Compiled inline: as a called function it
+// cost the rows that never come here a quarter of their time.)
+template <typename T, bool kE4M3>
+__device__ __forceinline__ void norm_past_range(const RowsParams& p, int64_t row, bool mine, float sum,
+                                             float (*s_sum)[32], uint32_t (*s_max)[32],
+                                             int parity) {
+  const int lanes = p.lanes, t = threadIdx.x % lanes;
+  const T* h = p.residual != nullptr ? static_cast<const T*>(p.h) + row * p.ldh
+                                     : static_cast<const T*>(p.x) + row * p.ldx;
+  auto values = [&](int c0, float factor, float (&u)[8], float& total) {
+    load_row8<T>(h, c0, p.cols).values(u);
+    float w[8];
+    if (p.weight_f32)
+      load_row8<float, true>(static_cast<const float*>(p.weight), c0, p.cols).values(w);
+    else
+      load_row8<T, true>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] *= factor;
+      total = fmaf(u[j], u[j], total);
+      u[j] *= w[j];
+    }
+  };
+  float factor = sum < __uint_as_float(kInfBits) ? 1.0f : 8.271806125530277e-25f;  // 2^-80
+  uint32_t most = 0;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    float total = 0.0f, big = 0.0f;
+#pragma unroll 1
+    for (int c0 = t * 8; mine && c0 < p.cols; c0 += lanes * 8) {
+      float u[8];
+      values(c0, factor, u, total);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
+    }
+    reduce_row<true>(lanes, total, big, most, s_sum[parity], s_max[parity]);
+    parity ^= 1;
+    if (turn == 0) factor *= rsqrtf(fmaf(total, p.inv_cols, p.eps * factor * factor));
+  }
+  if (!mine) return;
+  const Factor f = finish_row<false, kE4M3>(p, row, 0.0f, most, t == 0);
+#pragma unroll 1
+  for (int c0 = t * 8; c0 < p.cols; c0 += lanes * 8) {
+    float u[8] = {}, unused = 0.0f;
+    if (f.hi != 0.0f) values(c0, factor, u, unused);
+    store_codes<kE4M3, false>(p.q + row * p.ldq, c0, p.cols, p.codes_vec, u, f);
+  }
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -514,7 +565,7 @@ constexpr int thread_regs(int threads) { return 65536 / threads / 8 * 8; }
 // their rate (4096 x 8192 with a residual 54.9 us).
 template <typename T, Mode kMode, bool kE4M3, bool kWhole, bool kHeld>
 __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
-    rows8_staged_kernel(const RowsParams p) {
+    rows8_staged_kernel(const __grid_constant__ RowsParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_sum[2][32];
   __shared__ uint32_t s_max[2][32];
@@ -601,10 +652,6 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
     // in 16 bits is stored by store_shifted8).
     auto chunk = [&](int c0, auto start) {
       constexpr bool kStart = decltype(start)::value;
-      if constexpr (kEarly && !kStart) {  // the slot holds a later row by now
-        const uint8_t* from = kMode == kSummed ? at(p.h, row, p.sh) : at(p.x, row, p.sx);
-        return load8<T, false>(reinterpret_cast<const T*>(from) + c0);
-      }
       Eight<T> e = staged8<T, kWhole>(slot + off + c0 * kSize);
       if constexpr (kMode == kSummed && (kStart || kHeld || !kWhole)) {
         add<T>(e, staged8<T, kWhole>(slot + p.slot + offr + c0 * kSize));
@@ -623,7 +670,7 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
       return e;
     };
     // u = h * weight, the sum of h^2
-    auto values = [&](const Eight<T>& e, int c0, auto scaled, float (&u)[8], float& sum) {
+    auto values = [&](const Eight<T>& e, int c0, float (&u)[8], float& sum) {
       e.values(u);
       if (!kWhole && c0 + 8 > p.cols) {  // the row's last chunk
 #pragma unroll
@@ -637,7 +684,6 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
           load_weights<T, kWhole>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if constexpr (decltype(scaled)::value) u[j] *= kDown;
           sum = fmaf(u[j], u[j], sum);
           u[j] *= w[j];
         }
@@ -651,11 +697,13 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
     auto put = [&](int c0, const float (&u)[8], Factor f) {
       store_codes<kE4M3, kWhole>(q, c0, p.cols, p.codes_vec, u, f);
     };
-    auto quantize = [&](auto scaled, Factor f) {  // from the staged row
+    auto quantize = [&](Factor f) {  // from the staged row, or zeros
 #pragma unroll 2
       for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
         float u[8] = {}, unused = 0.0f;
-        if (f.hi != 0.0f) values(chunk(c0, std::false_type{}), c0, scaled, u, unused);
+        if constexpr (!kHeld) {
+          if (f.hi != 0.0f) values(chunk(c0, std::false_type{}), c0, u, unused);
+        }
         put(c0, u, f);
       }
     };
@@ -674,10 +722,10 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
           store_shifted8<T>(h, c0, cols, e, t == 0 || (t & 31) == 0,
                             t + 1 == lanes || (t & 31) == 31);
           if (c0 >= cols) continue;
-          values(e, c0, std::false_type{}, held[c], sum);
+          values(e, c0, held[c], sum);
           big = largest(big, held[c]);
         } else if (c0 < cols) {
-          values(chunk(c0, std::true_type{}), c0, std::false_type{}, held[c], sum);
+          values(chunk(c0, std::true_type{}), c0, held[c], sum);
           big = largest(big, held[c]);
         }
       }
@@ -685,32 +733,24 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
     } else {
 #pragma unroll 2
       for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
-        values(chunk(c0, std::true_type{}), c0, std::false_type{}, held[0], sum);
+        values(chunk(c0, std::true_type{}), c0, held[0], sum);
         big = largest(big, held[0]);
       }
     }
     reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
     parity ^= 1;
-    // once more, scaled: a warp with several rows goes together
+    // a warp with several rows goes together
     const bool again = live && past_range<kNorm>(sum, most);
-    if (kNorm && (lanes < 32 ? __any_sync(0xffffffffu, again) : again)) {
-      float sum2 = 0.0f, big2 = 0.0f;
-      uint32_t most2;
-#pragma unroll 1
-      for (int c0 = t * 8; again && c0 < cols; c0 += lanes * 8) {
-        float u[8];
-        values(chunk(c0, std::false_type{}), c0, std::true_type{}, u, sum2);
-        big2 = largest(big2, u);
+    if constexpr (kNorm) {
+      if (lanes < 32 ? __any_sync(0xffffffffu, again) : again) {
+        group_sync(lanes);  // threads may have stored values of h for one another
+        norm_past_range<T, kE4M3>(p, row, again, sum, s_sum, s_max, parity);
       }
-      reduce_row<kNorm>(lanes, sum2, big2, most2, s_sum[parity], s_max[parity]);
-      parity ^= 1;
-      if (again)
-        quantize(std::true_type{}, finish_row<kNorm, kE4M3>(p, row, sum2, most2, true, t == 0));
     }
     if (live && !again) {
-      const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, false, t == 0);
+      const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, t == 0);
       if (!kHeld || f.hi == 0.0f) {
-        quantize(std::false_type{}, f);
+        quantize(f);
       } else {
 #pragma unroll
         for (int c = 0; c < kHold; ++c) {
@@ -731,7 +771,7 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
 // sum are those of the staged kernel, whatever its width: a CTA of `lanes` threads,
 // or one warp of which `lanes` hold the row and the rest hold nothing.
 template <typename T, bool kNorm, bool kE4M3>
-__global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const __grid_constant__ RowsParams p) {
   __shared__ float s_sum[2][32];
   __shared__ uint32_t s_max[2][32];
   const int64_t row = blockIdx.x;
@@ -743,7 +783,7 @@ __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams 
   const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
   T* h = static_cast<T*>(p.h) + row * p.ldh;
   const bool residual = kNorm && p.residual != nullptr;
-  auto values = [&](bool start, float factor, int c0, float (&u)[8], float& sum) {
+  auto values = [&](bool start, int c0, float (&u)[8], float& sum) {
     Eight<T> e = load_row8<T>(residual && !start ? h : x, c0, p.cols);
     if (residual && start) {
       add<T>(e, load_row8<T>(r, c0, p.cols));
@@ -758,36 +798,32 @@ __global__ void __launch_bounds__(kMaxLanes) rows8_long_kernel(const RowsParams 
         load_row8<T, true>(static_cast<const T*>(p.weight), c0, p.cols).values(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        u[j] *= factor;
         sum = fmaf(u[j], u[j], sum);
         u[j] *= w[j];
       }
     }
   };
-  float sum, factor = 1.0f;
+  float sum = 0.0f, big = 0.0f;
   uint32_t most;
-  auto pass = [&](bool start, int parity) {
-    float big = 0.0f;
-    sum = 0.0f;
-    for (int c0 = begin; c0 < p.cols; c0 += lanes * 8) {
-      float u[8];
-      values(start, factor, c0, u, sum);
+  for (int c0 = begin; c0 < p.cols; c0 += lanes * 8) {
+    float u[8];
+    values(true, c0, u, sum);
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
-    }
-    reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);
-  };
-  pass(true, 0);
-  bool scaled = past_range<kNorm>(sum, most);
-  if (lanes < 32) scaled = __any_sync(0xffffffffu, scaled);  // the whole warp as the row
-  if (scaled) {
-    factor = kDown;
-    pass(false, 1);
+    for (int j = 0; j < 8; j += 2) big = max3_abs(big, u[j], u[j + 1]);
   }
-  const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, scaled, t == 0);
+  reduce_row<kNorm>(lanes, sum, big, most, s_sum[0], s_max[0]);
+  if constexpr (kNorm) {
+    bool again = past_range<kNorm>(sum, most);
+    if (lanes < 32) again = __any_sync(0xffffffffu, again);  // the whole warp as the row
+    if (again) {
+      norm_past_range<T, kE4M3>(p, row, t < lanes, sum, s_sum, s_max, 1);
+      return;
+    }
+  }
+  const Factor f = finish_row<kNorm, kE4M3>(p, row, sum, most, t == 0);
   for (int c0 = begin; c0 < p.cols; c0 += lanes * 8) {
     float u[8], unused = 0.0f;
-    values(false, factor, c0, u, unused);
+    values(false, c0, u, unused);
     if (f.hi == 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = 0.0f;

@@ -438,3 +438,23 @@ def test_rows_around_the_widest_that_threads_hold(cols, dt, residual):
         else:
             q, s = pk.rms_norm_quant(x, w, 1e-5, dtype=code)
         _check_codes(q, s, _norm64(h, w, 1e-5), 8, (80 / 2 + 8) * U)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("cols", [20, 64, 1001, 8192, 33000])
+def test_norm_of_products_past_fp32(cols, residual):
+    """h * w past fp32's range where h * r * w is not: the row's own sum and eps
+    count, whatever is done to reach the product."""
+    x = (_x(5, cols, torch.float32) * 0 + 1) * torch.linspace(-1, 1, cols, device="cuda") + 2.0
+    w = torch.linspace(0.5, 1, cols, device="cuda")
+    tol = (max(64, cols // 1024) / 2 + 16) * U
+    for size, weight, eps in ((1e3, 1e36, 1e-6), (1e3, 1e36, 1e6), (1.0, 2e38, 1e-6), (2.0 ** 65, 1.0, 2.0 ** 127),
+                              (2.0 ** 65, 1e30, 2.0 ** 127), (2.0 ** 100, 1e20, 1e-6)):
+        h = x * size
+        v = w * weight
+        if residual:
+            q, s, got = pk.rms_norm_quant(h * 0.5, v, eps, residual=h * 0.5)
+            assert torch.equal(got, h)
+        else:
+            q, s = pk.rms_norm_quant(h, v, eps)
+        _check_codes(q, s, _norm64(h, v, eps), 8, tol)
