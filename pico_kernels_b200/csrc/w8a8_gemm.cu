@@ -13,7 +13,8 @@
 //    The product is a weight stream there (16 x 28672 x 8192: 38 us = 6.2 TB/s);
 //    K is split over a thread-block cluster when there are too few column tiles
 //    to keep every SM loading, and the partial sums meet in distributed shared
-//    memory (in rank order; no workspace, no atomics).
+//    memory (in rank order; no workspace, no atomics). A CTA gives its tensor
+//    memory back before it waits for the others of its cluster.
 //  * w8a8_pair_kernel, many tokens: persistent, 256 x 256 tiles of a CTA pair
 //    (cta_group::2), two accumulators so that a tile's epilogue overlaps the
 //    next one's main loop (4096 x 11008 x 4096 int8: 117 us = 3.2 POP/s, the
@@ -46,7 +47,7 @@ struct Params {
   int out_dtype, act;
   int rows16;        // the output's rows start on 16-byte boundaries
   // swap: CTAs per tile along K (the cluster), tokens of a tile (a multiple of
-  // 16), the ring, TMEM columns, whether the sums of a split have their own memory
+  // 16), the ring, TMEM columns, whether a split's sums have memory beside the ring
   int split, nt, stages, stage_bytes, tmem_cols, own_red;
   int pieces;        // swap: accumulators that a CTA's K range is summed in
   int num_m, num_n;  // tiles
@@ -236,13 +237,17 @@ __global__ void __launch_bounds__(kThreads)
       if (kGated) tma_prefetch_l2_2d(&tmW1, kt * kBK, n0);
     }
   }
+  // Memory beside the ring takes sums from CTAs that know of its owner's start. The
+  // word goes out before the wait for tensor memory, so that whoever holds some
+  // waits for nothing but its own loads and MMAs: clusters of several streams that
+  // share SMs then cannot hold on one of them what the other needs on the next.
+  __syncwarp();
+  if (p.own_red) cluster_arrive_unordered();
   if (warp == kMmaWarp) tmem_alloc(tmem_holder, p.tmem_cols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  // a CTA's own memory for sums takes them from a CTA that has started
-  if (p.own_red && p.split > 1) cluster_sync();
   griddep_wait();
   griddep_launch_dependents();
 
@@ -379,17 +384,15 @@ __global__ void __launch_bounds__(kThreads)
       });
     }
   } else {
-    // Rank r of the cluster owns tokens [r * per, (r + 1) * per): every CTA
-    // stores its sums of them into r's memory, then r adds the ranks' sums in
-    // order. One cluster barrier in between (and one before, where the memory
-    // is the ring: its owner's MMAs are then done).
+    // Rank r of the cluster owns tokens [r * per, (r + 1) * per) and adds the ranks'
+    // sums of them in order. Sums that have memory beside the ring are stored into
+    // the owner's, more of them into this CTA's own drained ring, from where their
+    // owner fetches them.
     const int per = (tokens + p.split - 1) / p.split;
-    if (!p.own_red) {
-      __syncwarp();
-      cluster_sync();
-    }
     const uint32_t red = smem_u32(
         p.own_red ? smem + stages * stage_bytes + kMaxTokens * 4 + kSwapBars : smem);
+    __syncwarp();
+    if (p.own_red) cluster_wait();
     if (epi && !fail) {
 #pragma unroll 1
       for (int c = part * (nt / 2); c < (part + 1) * (nt / 2) && c < tokens; c += 8) {
@@ -398,6 +401,12 @@ __global__ void __launch_bounds__(kThreads)
           uint32_t x[8];
           load_sums(w * nt + c, x);
           tmem_ld_wait();
+          if (!p.own_red) {  // [token][weight][channel]
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              sts_f32(red + ((c + i) * kW + w) * 512 + nl * 4, __uint_as_float(x[i]));
+            continue;
+          }
           int owner = c / per, at = c - owner * per;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -414,28 +423,33 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
+    // the sums are where they are read; this CTA's tensor memory goes back before it
+    // waits for the others
     __syncwarp();
-    cluster_sync();
-    if (epi && !fail) {
-      const int first = ks * per;
+    cluster_arrive();
+    tc_fence_before();
+    fail = __syncthreads_or(fail);
+    if (fail) drain();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, p.tmem_cols);
+    __syncwarp();
+    const int first = ks * per, last = min(first + per, tokens);
+    auto add = [&](float a, float b) {
+      return kE4M3 ? a + b : __uint_as_float(__float_as_uint(a) + __float_as_uint(b));
+    };
+    auto value = [&](float sum) { return acc_value<kE4M3>(__float_as_uint(sum)); };
+    if (p.own_red) {
+      cluster_wait();
+      if (!epi || fail) return;
       auto total = [&](int m, int w) {
         const uint32_t at = red + (((m - first) * kW + w) * p.split) * 512 + ch * 4;
-        if constexpr (kE4M3) {
-          float v = lds_f32(at);
+        float v = lds_f32(at);
 #pragma unroll
-          for (int j = 1; j < kMaxSplit; ++j)
-            if (j < p.split) v += lds_f32(at + j * 512);
-          return v;
-        } else {
-          uint32_t v = lds_u32(at);
-#pragma unroll
-          for (int j = 1; j < kMaxSplit; ++j)
-            if (j < p.split) v += lds_u32(at + j * 512);
-          return static_cast<float>(static_cast<int>(v));
-        }
+        for (int j = 1; j < kMaxSplit; ++j)
+          if (j < p.split) v = add(v, lds_f32(at + j * 512));
+        return value(v);
       };
       with_type(p.out, p.out_dtype, [&](auto* out) {
-        const int last = min(first + per, tokens);
         // four tokens (of this thread's parity) at a time, read before stored
 #pragma unroll 1
         for (int m = first + (et >> 7); m < last; m += 8) {
@@ -452,7 +466,79 @@ __global__ void __launch_bounds__(kThreads)
             if (inside && m + 2 * i < last) put(o, v[i]);
         }
       });
+      return;
     }
+    // Four channels a thread, eight tokens at a time: every rank's sums of a token on
+    // their way before the first is added (128 x 4096 x 4096 9.4 us, by single words
+    // 13.5).
+    const int c4 = (et & 31) * 4, n4 = n0 + c4;
+    float s4[kW][4], b4[4];
+    if (epi) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int w = 0; w < kW; ++w) s4[w][e] = n4 + e < p.N ? p.w_scale[w][n4 + e] : 0.0f;
+        b4[e] = biased && n4 + e < p.N ? p.bias[n4 + e] : 0.0f;
+      }
+    }
+    cluster_wait();
+    if (epi && !fail) {
+      auto total4 = [&](int m, int w, float (&v)[4]) {
+        const uint32_t at = red + (m * kW + w) * 512 + c4 * 4;
+        uint4 x[kMaxSplit];
+#pragma unroll
+        for (int j = 0; j < kMaxSplit; ++j)
+          if (j < p.split) x[j] = ld_cluster_v4(cluster_map(at, j));
+        float4 t = make_float4(__uint_as_float(x[0].x), __uint_as_float(x[0].y),
+                               __uint_as_float(x[0].z), __uint_as_float(x[0].w));
+#pragma unroll
+        for (int j = 1; j < kMaxSplit; ++j) {
+          if (j < p.split) {
+            t.x = add(t.x, __uint_as_float(x[j].x));
+            t.y = add(t.y, __uint_as_float(x[j].y));
+            t.z = add(t.z, __uint_as_float(x[j].z));
+            t.w = add(t.w, __uint_as_float(x[j].w));
+          }
+        }
+        v[0] = value(t.x);
+        v[1] = value(t.y);
+        v[2] = value(t.z);
+        v[3] = value(t.w);
+      };
+#pragma unroll 1
+      for (int m = first + (et >> 5); m < last; m += 8) {
+        const float sa = lds_f32(sa_addr + m * 4);
+        float v[4], g[4];
+        total4(m, 0, v);
+        if constexpr (kGated) total4(m, kW - 1, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = v[e] * sa * s4[0][e];
+          if constexpr (kGated) v[e] = gated(v[e], g[e] * sa * s4[kW - 1][e], p.act);
+          else if (biased) v[e] += b4[e];
+        }
+        const int64_t at = static_cast<int64_t>(m0 + m) * p.ldo + n4;
+        if (p.rows16 && n4 + 4 <= p.N) {
+          if (p.out_dtype == PK_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) =
+                make_float4(v[0], v[1], v[2], v[3]);
+          else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(
+                pack16(p.out_dtype, v[0], v[1]), pack16(p.out_dtype, v[2], v[3]));
+        } else {
+          with_type(p.out, p.out_dtype, [&](auto* out) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n4 + e < p.N) put(out + at + e, v[e]);
+          });
+        }
+      }
+    }
+    // no CTA leaves while another fetches from its ring
+    __syncwarp();
+    cluster_arrive_unordered();
+    cluster_wait();
+    return;
   }
 
   tc_fence_before();
@@ -847,14 +933,6 @@ SwapSmem swap_smem(const Plan& plan, bool gated, int64_t k_tiles) {
   c.bytes = c.stages * c.stage_bytes + rest;
   c.tmem_cols = 32;
   while (c.tmem_cols < plan.nt * w * plan.pieces) c.tmem_cols *= 2;
-  // CTAs of a cluster wait for one another with their tensor memory held. Two
-  // clusters of different streams that share two SMs must therefore never ask
-  // for more of it than there is, or each may hold on one SM what the other
-  // waits for on the other: a CTA of a split takes at least the share of the
-  // SM's 228 KB (1 KB a CTA is the system's) that its columns are of the 512,
-  // and no less than 40 KB, which leaves it no room beside a kernel that takes
-  // all 512 columns with 194 KB of its own.
-  if (plan.split > 1) c.bytes = std::max({c.bytes, c.tmem_cols * (228 * 1024 / 512) - 1024, 40 * 1024});
   return c;
 }
 

@@ -384,3 +384,63 @@ def test_products_of_several_streams_at_once():
             for k, y in rows:
                 assert torch.equal(y.nan_to_num(), want[k].nan_to_num()), sizes[k // 4]
     assert pk.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 515, 4096), (33, 130, 8192), (50, 1, 8192), (64, 515, 4096),
+                                   (100, 1000, 8192), (112, 260, 4000), (144, 130, 16384),
+                                   (250, 513, 8192), (256, 1024, 8192)])
+def test_sums_of_a_split_that_their_owners_fetch(M, N, K):
+    """Few channel tiles and long sums: K is split over a cluster, more sums than the
+    memory beside the ring holds. Ragged tokens and channels, rows of outputs on and
+    off 16-byte boundaries."""
+    for code in CODES:
+        a, sa, (wg, sg, wu, su), b = _operands(M, N, K, code, seed=3, weights=2)
+        (g, eg), (u, eu) = _product64(a, sa, wg, sg), _product64(a, sa, wu, su)
+        y = pk.w8a8_gemm(a, sa, wg, sg, bias=b)
+        _assert_near(y, g + b.double(), eg + U * (g.abs() + b.double().abs()))
+        f, t = _act64(g, "silu")
+        ref = f * u
+        z = pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su)
+        _assert_near(z, ref, 1.2 * eg * (u.abs() + eu) + f.abs() * eu +
+                     (12 + 4 * (-t).clamp(0, 100)) * U * ref.abs(), 1e-5)
+        if code == torch.int8:
+            for dt in (torch.bfloat16, torch.float16):
+                assert torch.equal(pk.w8a8_gemm(a, sa, wg, sg, bias=b, out_dtype=dt), y.to(dt))
+                assert torch.equal(pk.w8a8_gated_gemm(a, sa, wg, sg, wu, su, out_dtype=dt), z.to(dt))
+    assert pk.device_status() == (0, 0)
+
+
+def test_split_products_beside_the_other_kernels_of_tensor_memory():
+    """Clusters of 32 to 512 columns a CTA on one stream, single CTAs, pairs and the
+    int4 decode kernel on others: whoever waits for another CTA of a cluster holds no
+    tensor memory that a third one needs. Results as of the calls one by one."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    calls = [[], [], []]
+    for i, (M, N, K, s) in enumerate([(1, 512, 8192, 0), (16, 384, 16384, 0), (40, 512, 8192, 0),
+                                      (100, 640, 8192, 0), (144, 256, 16384, 0), (256, 512, 8192, 0),
+                                      (1, 640, 16384, 1), (130, 512, 8192, 1), (300, 2048, 1024, 1),
+                                      (64, 512, 4096, 1), (1000, 2000, 512, 1), (24, 1024, 4096, 1)]):
+        code = CODES[i & 1]
+        a, w, u = (_codes(r, K, code, g) for r in (M, N, N))
+        sa, sw = (torch.rand(r, device="cuda", generator=g) / 1000 for r in (M, N))
+        calls[s].append(lambda a=a, sa=sa, w=w, sw=sw: pk.w8a8_gemm(a, sa, w, sw))
+        calls[s].append(lambda a=a, sa=sa, w=w, sw=sw, u=u: pk.w8a8_gated_gemm(a, sa, w, sw, u, sw))
+    w4, scales = pk.quantize_int4_grouped(torch.randn(4096, 1024, device="cuda", generator=g), 128,
+                                          torch.bfloat16)
+    for M in (16, 32):
+        x = torch.randn(M, 4096, device="cuda", generator=g).bfloat16()
+        calls[2].append(lambda x=x: pk.int4_gemm(x, w4, scales, group_size=128))
+    want = [[f() for f in c] for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for turn in range(30):
+        for c, stream, out in zip(calls, streams, got):
+            with torch.cuda.stream(stream):
+                for j in range(6):
+                    k = (turn * 5 + j) % len(c)
+                    out.append((k, c[k]()))
+    torch.cuda.synchronize()
+    for out, ref in zip(got, want):
+        assert all(torch.equal(y, ref[k]) for k, y in out)
+    assert pk.device_status() == (0, 0)
