@@ -1008,7 +1008,8 @@ cudaError_t launch_pair(const W8A8Args& g, cudaStream_t s, const char** why) {
 //    SM 148, of clusters of 4 132, of clusters of 8 120;
 //  * swap: 2.5 us of launch and first loads, 0.7 more where a CTA takes most of an
 //    SM's memory (the next kernel's CTAs then wait for it); per token of a tile
-//    13 ns of epilogue (gated 23), with a K split 0.4 us + nt * (30 + 20 / split) ns;
+//    13 ns of epilogue (gated 23), with a K split 0.8 us + nt * (5 + 40 / split) ns a
+//    weight;
 //  * pair: 6 us around the main loop, 0.28 us a K tile (0.21 of a half unit, 0.155
 //    of a quarter).
 constexpr float kSmBytes = 150e3f, kHbmBytes = 6.3e6f, kLatency = 1.6f;  // per us; us
@@ -1052,7 +1053,7 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
   };
   const float epilogue = plan.split == 1
                              ? nt * (g.gated ? 0.023f : 0.013f)
-                             : 0.4f + w * nt * (0.030f + 0.020f / split);
+                             : 0.8f + w * nt * (0.005f + 0.040f / split);
   // two CTAs on an SM: a fifth of an epilogue hides behind the other's
   const int64_t full = ctas / (one * occ), rest = ctas % (one * occ);
   float us = (c.bytes > kMaxSmem / 2 ? 3.2f : 2.5f) +
