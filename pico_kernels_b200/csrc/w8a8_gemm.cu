@@ -1064,33 +1064,30 @@ float plan_us(const Plan& plan, const W8A8Args& g) {
 
 // An e4m3 MMA loses a part of its accumulator's last place at each step, always
 // towards zero: measured 4.5e-9 of the result a step of 32, 1e-6 after 7168 of
-// K. Where the output is fp32, no accumulator takes more than kPiece K tiles:
-// the K splits and pieces of a swap CTA are added up in fp32 instead. Against a
-// 16-bit output's rounding (2^-9 at best) the loss is nothing.
-constexpr int kPiece = 40;
+// K. So an accumulator takes a limited number of K tiles, and the K splits and
+// pieces of a swap CTA are added up in fp32: 40 tiles (7e-7) where the output is fp32,
+// 1280 (2.3e-5, a twentieth of fp16's half step) where it has 16 bits. A tile of 16
+// tokens holds 32 accumulators a CTA (gated 16) in a split of 8: fp32 outputs of more
+// than 1310720 of K (gated 655360) have longer pieces, evenly. The pair kernel has one
+// accumulator.
+constexpr int kPieceF32 = 40, kPiece16 = 1280;
 
 Plan search(const W8A8Args& g) {
   const int64_t k_tiles = ceil_div(g.K, kBK);
-  const bool pieces = g.e4m3 && g.out_dtype == PK_F32;
+  const int64_t limit = !g.e4m3 ? k_tiles : g.out_dtype == PK_F32 ? kPieceF32 : kPiece16;
   Plan best{true, 0, 1, false, 1};
-  float least = g.M > 128 && !(pieces && k_tiles > kPiece) ? plan_us(best, g) : 1e30f;
-  int64_t fewest = 1ll << 60;  // K tiles over kPiece in an accumulator, 0 before all else
+  float least = g.M > 128 && k_tiles <= limit ? plan_us(best, g) : 1e30f;
+  int64_t fewest = 1ll << 60;  // K tiles over the limit in an accumulator, 0 before all else
   if (least < 1e30f) fewest = 0;
-  // token tiles as even as sixteens allow, from as few as there can be to 16 wide
-  for (int64_t num_m = ceil_div(g.M, kMaxTokens), nt = 0, last = 0; num_m <= ceil_div(g.M, 256) + 16;
-       ++num_m) {
-    nt = ceil_div(ceil_div(g.M, num_m), 16) * 16;
-    if (nt == last) continue;
-    last = nt;
+  auto consider = [&](int nt) {
     for (int split = 1; split <= kMaxSplit && split <= k_tiles; split *= 2) {
       for (int deep = 0; deep < 2; ++deep) {
-        Plan plan{false, static_cast<int>(nt), split, deep != 0, 1};
+        Plan plan{false, nt, split, deep != 0, 1};
         if (!swap_smem(plan, g.gated, k_tiles).fits) continue;
         const int64_t kt = ceil_div(k_tiles, split);
         const int cols = plan.nt * (g.gated ? 2 : 1);
-        if (pieces)
-          while (plan.pieces * kPiece < kt && 2 * plan.pieces * cols <= (deep ? 512 : 256)) plan.pieces *= 2;
-        const int64_t over = pieces ? std::max<int64_t>(0, ceil_div(kt, plan.pieces) - kPiece) : 0;
+        while (plan.pieces * limit < kt && 2 * plan.pieces * cols <= (deep ? 512 : 256)) plan.pieces *= 2;
+        const int64_t over = std::max<int64_t>(0, ceil_div(kt, plan.pieces) - limit);
         const float us = plan_us(plan, g);
         if (over < fewest || (over == fewest && us < least)) {
           fewest = over;
@@ -1099,8 +1096,17 @@ Plan search(const W8A8Args& g) {
         }
       }
     }
-    if (nt == 16) break;
+  };
+  // token tiles as even as sixteens allow, from as few as there can be to 16 wide
+  int last = 0;
+  for (int64_t num_m = ceil_div(g.M, kMaxTokens); num_m <= ceil_div(g.M, 256) + 16 && last != 16;
+       ++num_m) {
+    const int nt = static_cast<int>(ceil_div(ceil_div(g.M, num_m), 16) * 16);
+    if (nt != last) consider(nt);
+    last = nt;
   }
+  // the narrower, the more accumulators
+  while (fewest > 0 && last > 16) consider(last -= 16);
   return best;
 }
 

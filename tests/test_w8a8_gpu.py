@@ -444,3 +444,50 @@ def test_split_products_beside_the_other_kernels_of_tensor_memory():
     for out, ref in zip(got, want):
         assert all(torch.equal(y, ref[k]) for k, y in out)
     assert pk.device_status() == (0, 0)
+
+
+def _long_product64(a, sa, w, sw):
+    """_product64's value, K in pieces."""
+    y = sum(a[:, k:k + 65536].double() @ w[:, k:k + 65536].double().t()
+            for k in range(0, a.shape[1], 65536))
+    return y * (sa.double()[:, None] * sw.double())
+
+
+def _long_operands(M, N, K, weights):
+    g = torch.Generator(device="cuda").manual_seed(K)
+
+    def codes(rows):
+        t = torch.empty(rows, K, device="cuda", dtype=torch.float8_e4m3fn)
+        for k in range(0, K, 1 << 20):
+            n = min(1 << 20, K - k)
+            t[:, k:k + n] = (torch.randn(rows, n, device="cuda", generator=g) * 112).clamp_(-448, 448)
+        return t
+    s = [(0.5 + torch.rand(n, device="cuda", generator=g)) / 112 for n in (M, N, N)]
+    return codes(M), s[0], [t for i in range(weights) for t in (codes(N), s[1 + i] / K ** 0.5)]
+
+
+@pytest.mark.parametrize("weights", [1, 2])
+def test_long_e4m3_sums_of_many_tokens_keep_fp32_precision(weights):
+    # the bound of test_long_e4m3_sums_keep_fp32_precision for more tokens than the
+    # accumulators of one wide tile could hold in pieces of 5120
+    a, sa, w = _long_operands(2048, 128, 600000, weights)
+    ref = _long_product64(a, sa, w[0], w[1])
+    if weights == 1:
+        y = pk.w8a8_gemm(a, sa, *w)
+    else:
+        ref = _act64(ref, "silu")[0] * _long_product64(a, sa, w[2], w[3])
+        y = pk.w8a8_gated_gemm(a, sa, *w)
+    assert (torch.linalg.norm(y.double() - ref) <= 1e-6 * weights * torch.linalg.norm(ref)).item()
+
+
+def test_the_longest_e4m3_sums_keep_16_bit_precision():
+    # An output is off by half a step, 2^-11 of itself at most, and by what its
+    # accumulators truncate: 1280 K tiles of 4 steps each at 4.5e-9 of the result a
+    # step as measured, 2.4e-5, a twentieth of that. One accumulator for all of K
+    # would truncate 2.4e-3.
+    for M in (4, 130):
+        a, sa, w = _long_operands(M, 64, 1 << 24, 1)
+        ref = _long_product64(a, sa, *w)
+        y = pk.w8a8_gemm(a, sa, *w, out_dtype=torch.float16)
+        assert (torch.linalg.norm(y.double() - ref) <= 1.1 * 2.0 ** -11 * torch.linalg.norm(ref)).item()
+    assert pk.device_status() == (0, 0)
