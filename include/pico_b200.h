@@ -373,8 +373,8 @@ PK_API int pk_gemm_splitk(const void* a, const void* b, int dtype, int64_t M, in
 /* No counterparts in the reference. 8-bit operands (dtype I8 or E4M3) are
  * rows of K consecutive codes, `ld` codes apart, with x ~= code * scale[row]:
  * activations one row per token, weights [N, K] one row per output channel
- * (nn.Linear's own layout). Every pointer is aligned to its element. None of
- * them needs a workspace, so calls on different streams may overlap and
+ * (nn.Linear's own layout). Every pointer is aligned to its element, and outputs
+ * overlap no operand (but for h of the norm, below). None of them needs a workspace, so calls on different streams may overlap and
  * captured graphs share nothing; like the other calls they can be captured
  * after one eager call per shape. */
 

@@ -24,6 +24,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <utility>
 
 #include "pico_b200.h"
@@ -399,6 +400,22 @@ bool codes(PyObject* o, Codes* c) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// Whether two ranges of addresses meet.
+struct Range {
+  uintptr_t at;
+  int64_t bytes;
+};
+bool meet(Range a, Range b) { return a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+Range range_of(const at::Tensor& t) {  // contiguous
+  return {reinterpret_cast<uintptr_t>(t.data_ptr()), static_cast<int64_t>(t.nbytes())};
+}
+Range range_of(const Codes& c) {
+  return {reinterpret_cast<uintptr_t>(c.t->data_ptr()), (c.rows - 1) * c.pitch + c.K};
+}
+Range range_of(const float* p, int64_t n) {
+  return {reinterpret_cast<uintptr_t>(p), p != nullptr ? 4 * n : 0};
+}
+
 // dequantize_rows(codes, scale, dtype) -> values, or the status, or -1
 PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 3) {
@@ -454,9 +471,9 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (r == nullptr || o == nullptr || o->scalar_type() != x->scalar_type() ||
           o->sizes() != x->sizes() || !o->is_contiguous())
         return PyLong_FromLong(kNotServed);
-      // x, residual or a storage of its own: a partial overlap is refused in Python
+      // x, residual or memory of its own: another overlap is refused in Python
       for (const at::Tensor* in : {x, r, w})
-        if (o->is_alias_of(*in) && (in == w || o->data_ptr() != in->data_ptr()))
+        if (meet(range_of(*o), range_of(*in)) && (in == w || o->data_ptr() != in->data_ptr()))
           return PyLong_FromLong(kNotServed);
       h = *o;
     } else if (r != nullptr) {
@@ -485,9 +502,10 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// The output of a product: allocated, or `out_obj` (contiguous [M, N]).
+// The output of a product: allocated, or `out_obj` (contiguous [M, N]), which meets
+// none of the operands.
 bool product_out(PyObject* dtype_obj, PyObject* out_obj, int64_t M, int64_t N,
-                 const at::Tensor& like, at::Tensor* y) {
+                 const at::Tensor& like, std::initializer_list<Range> operands, at::Tensor* y) {
   at::ScalarType t;
   if (!dtype_arg(dtype_obj, &t) || code_of(t) < 0) return false;
   if (out_obj == Py_None) {
@@ -498,6 +516,8 @@ bool product_out(PyObject* dtype_obj, PyObject* out_obj, int64_t M, int64_t N,
   if (o == nullptr || o->scalar_type() != t || o->dim() != 2 || o->size(0) != M ||
       o->size(1) != N || !o->is_contiguous())
     return false;
+  for (const Range& r : operands)
+    if (meet(range_of(*o), r)) return false;
   *y = *o;
   return true;
 }
@@ -524,7 +544,10 @@ PyObject* w8a8_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const float* bias = args[4] == Py_None ? nullptr : row_values(args[4], w.rows);
     at::Tensor y;
     if (sa == nullptr || sw == nullptr || (args[4] != Py_None && bias == nullptr) ||
-        !product_out(args[5], args[6], a.rows, w.rows, *a.t, &y))
+        !product_out(args[5], args[6], a.rows, w.rows, *a.t,
+                     {range_of(a), range_of(sa, a.rows), range_of(w), range_of(sw, w.rows),
+                      range_of(bias, w.rows)},
+                     &y))
       return PyLong_FromLong(kNotServed);
     const int st = pk_w8a8_gemm(a.t->data_ptr(), a.code, a.pitch, sa, w.t->data_ptr(), w.pitch, sw,
                                 bias, a.rows, w.rows, a.K, y.data_ptr(), code_of(y.scalar_type()),
@@ -555,7 +578,10 @@ PyObject* w8a8_gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor y;
     if (sa == nullptr || sg == nullptr || su == nullptr ||
         (act != PK_ACT_SILU && act != PK_ACT_GELU_TANH) ||
-        !product_out(args[7], args[8], a.rows, g.rows, *a.t, &y))
+        !product_out(args[7], args[8], a.rows, g.rows, *a.t,
+                     {range_of(a), range_of(sa, a.rows), range_of(g), range_of(sg, g.rows),
+                      range_of(u), range_of(su, g.rows)},
+                     &y))
       return PyLong_FromLong(kNotServed);
     const int st = pk_w8a8_gated_gemm(a.t->data_ptr(), a.code, a.pitch, sa, g.t->data_ptr(),
                                       g.pitch, sg, u.t->data_ptr(), u.pitch, su,

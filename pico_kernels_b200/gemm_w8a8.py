@@ -78,6 +78,18 @@ def row_pitch(K: int) -> int:
     return (K + 15) // 16 * 16
 
 
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t: torch.Tensor) -> tuple[int, int]:
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.int8
                   ) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantize ``x[..., K]`` (fp16, bf16 or fp32) to 8 bits, one scale per row.
@@ -169,7 +181,7 @@ def _codes(t: torch.Tensor, dtype: torch.dtype | None, what: str) -> tuple[torch
 
 
 def _out(M: int, N: int, out_dtype: torch.dtype, out: torch.Tensor | None,
-         device: torch.device) -> torch.Tensor:
+         device: torch.device, operands) -> torch.Tensor:
     if out_dtype not in _FLOATS:
         raise _lib.DtypeError(f"output must be fp32, bf16 or fp16 (got {out_dtype})")
     if out is None:
@@ -178,6 +190,8 @@ def _out(M: int, N: int, out_dtype: torch.dtype, out: torch.Tensor | None,
             or not out.is_contiguous()):
         raise _lib.ShapeError(f"out must be a contiguous [{M}, {N}] {out_dtype} tensor on "
                               f"{device}")
+    if any(t is not None and overlaps(out, t) for t in operands):
+        raise _lib.ShapeError("out must not overlap an operand: they are read while it is written")
     return out
 
 
@@ -191,7 +205,7 @@ def w8a8_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale
     ``a_scale[M]``, ``w_scale[N]`` and ``bias[N]`` fp32. The scales and the
     bias are applied in fp32 in the epilogue and the result rounded once to
     ``out_dtype`` (fp32, bf16 or fp16), into ``out`` when given (a contiguous
-    ``[M, N]`` tensor of ``out_dtype``). No workspace and no host
+    ``[M, N]`` tensor of ``out_dtype`` that overlaps no operand). No workspace and no host
     synchronisation: calls can be captured in CUDA graphs.
     """
     tf = _lib.torch_fast()
@@ -211,7 +225,7 @@ def w8a8_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale
     sa = _scale(a_scale, (M,), a, "a_scale")
     sw = _scale(w_scale, (N,), a, "w_scale")
     b = None if bias is None else _scale(bias, (N,), a, "bias")
-    y = _out(M, N, out_dtype, out, a.device)
+    y = _out(M, N, out_dtype, out, a.device, (a, sa, w, sw, b))
     if y.numel() == 0:
         return y
     with _lib.on_device(a):
@@ -259,7 +273,7 @@ def w8a8_gated_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w_gate: torch.Tenso
     sa = _scale(a_scale, (M,), a, "a_scale")
     sg = _scale(gate_scale, (N,), a, "gate_scale")
     su = _scale(up_scale, (N,), a, "up_scale")
-    y = _out(M, N, out_dtype, out, a.device)
+    y = _out(M, N, out_dtype, out, a.device, (a, sa, g, sg, u, su))
     if y.numel() == 0:
         return y
     with _lib.on_device(a):

@@ -8,25 +8,14 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .gemm_w8a8 import _FLOATS, as_rows, check_codes_dtype, check_rows, empty_rows, row_pitch
+from .gemm_w8a8 import (_FLOATS, as_rows, check_codes_dtype, check_rows, empty_rows, overlaps,
+                        row_pitch)
 
 __all__ = ["rms_norm_quant"]
 
 
 def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
-
-
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
-    def span(t: torch.Tensor) -> tuple[int, int]:
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
@@ -75,8 +64,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
             raise _lib.ShapeError(f"residual_out must be a contiguous {tuple(x.shape)} {x.dtype} "
                                   f"tensor on {x.device}")
         if residual_out is not None and (
-                _overlaps(residual_out, weight)
-                or any(_overlaps(residual_out, t) and not _same(residual_out, t)
+                overlaps(residual_out, weight)
+                or any(overlaps(residual_out, t) and not _same(residual_out, t)
                        for t in (x, residual))):
             raise _lib.ShapeError("residual_out may be x or residual itself, but not overlap "
                                   "them otherwise")

@@ -229,3 +229,27 @@ def test_linear_keeps_its_types(code):
     loaded = pk.W8A8Linear(20, 6, dtype=code).half()
     loaded.load_state_dict(layer.state_dict())
     assert torch.equal(loaded.scales, scales)
+
+
+def test_outputs_that_overlap_an_operand_are_refused(as_if_on_a_gpu):
+    pool = torch.zeros(4096, dtype=torch.uint8)
+    q = pool[:1024].view(torch.int8).view(32, 32)
+    s, b = (pool[i:i + 128].view(torch.float32) for i in (1024, 1152))
+    w, one = torch.zeros(32, 32, dtype=torch.int8), torch.ones(32)
+
+    def out(at):
+        return pool[at:at + 2048].view(torch.bfloat16).view(32, 32)
+
+    bf = torch.bfloat16
+    for at, a8, sa, w8, sw, bias in ((0, q, one, w, one, None), (1022, q, one, w, one, None),
+                                     (0, w, one, q, one, None), (1022, w, one, q, one, None),
+                                     (1024, w, s, w, one, None), (1150, w, one, w, s, None),
+                                     (1152, w, one, w, one, b), (1278, w, one, w, one, b)):
+        with pytest.raises(_lib.ShapeError):
+            pk.w8a8_gemm(a8, sa, w8, sw, bias=bias, out_dtype=bf, out=out(at))
+        if bias is None:
+            for weights in ((w8, sw, w, one), (w, one, w8, sw)):
+                with pytest.raises(_lib.ShapeError):
+                    pk.w8a8_gated_gemm(a8, sa, *weights, out_dtype=bf, out=out(at))
+    with pytest.raises(AssertionError):  # not refused: it gets to its launch
+        pk.w8a8_gemm(q, s, w, one, bias=b, out_dtype=bf, out=out(1280))

@@ -491,3 +491,38 @@ def test_the_longest_e4m3_sums_keep_16_bit_precision():
         y = pk.w8a8_gemm(a, sa, *w, out_dtype=torch.float16)
         assert (torch.linalg.norm(y.double() - ref) <= 1.1 * 2.0 ** -11 * torch.linalg.norm(ref)).item()
     assert pk.device_status() == (0, 0)
+
+
+def test_out_beside_and_over_operands():
+    """Memory next to an operand is served, an overlap refused, on both paths."""
+    M, N, K = 32, 48, 64
+    a, sa, (w, sw, u, su), b = _operands(M, N, K, torch.int8, weights=2)
+    sizes = [t.numel() * t.element_size() for t in (a, sa, w, sw, u, su, b)]
+    pool = torch.zeros(sum(sizes) + 2 * M * N * 2, device="cuda", dtype=torch.uint8)
+    views, at = [], 0
+    for t, n in zip((a, sa, w, sw, u, su, b), sizes):
+        views.append(pool[at:at + n].view(t.dtype).view(t.shape).copy_(t))
+        at += n
+    want = (pk.w8a8_gemm(a, sa, w, sw, bias=b, out_dtype=torch.bfloat16),
+            pk.w8a8_gated_gemm(a, sa, w, sw, u, su, out_dtype=torch.bfloat16))
+    va, vsa, vw, vsw, vu, vsu, vb = views
+
+    def out(at):
+        return pool[at:at + M * N * 2].view(torch.bfloat16).view(M, N)
+
+    saved = _lib._tfast
+    for fast in (saved, False):
+        _lib._tfast = fast
+        try:
+            y = pk.w8a8_gemm(va, vsa, vw, vsw, bias=vb, out_dtype=torch.bfloat16, out=out(at))
+            z = pk.w8a8_gated_gemm(va, vsa, vw, vsw, vu, vsu, out_dtype=torch.bfloat16,
+                                   out=out(at + M * N * 2))
+            assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+            for i in range(len(sizes)):  # ends at, or starts in, an operand's last bytes
+                o = out(max(0, sum(sizes[:i + 1]) - 4))
+                with pytest.raises(_lib.ShapeError):
+                    pk.w8a8_gemm(va, vsa, vw, vsw, bias=vb, out_dtype=torch.bfloat16, out=o)
+            with pytest.raises(_lib.ShapeError):
+                pk.w8a8_gated_gemm(va, vsa, vw, vsw, vu, vsu, out_dtype=torch.bfloat16, out=out(0))
+        finally:
+            _lib._tfast = saved
