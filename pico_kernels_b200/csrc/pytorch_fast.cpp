@@ -400,6 +400,12 @@ bool codes(PyObject* o, Codes* c) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// Tells autograd that a caller's tensor has new contents (a backward pass that saved
+// the old ones then fails; inference tensors are not counted).
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Whether two ranges of addresses meet.
 struct Range {
   uintptr_t at;
@@ -489,6 +495,7 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (st != PK_OK) return PyLong_FromLong(st);
     PyObject* ho = nullptr;
     if (args[5] != Py_None) {
+      written(h);
       Py_INCREF(args[5]);
       ho = args[5];
     } else if (r != nullptr) {
@@ -525,6 +532,7 @@ bool product_out(PyObject* dtype_obj, PyObject* out_obj, int64_t M, int64_t N,
 PyObject* product_result(int st, PyObject* out_obj, at::Tensor&& y) {
   if (st != PK_OK) return PyLong_FromLong(st);
   if (out_obj == Py_None) return THPVariable_Wrap(std::move(y));
+  written(y);
   Py_INCREF(out_obj);
   return out_obj;
 }

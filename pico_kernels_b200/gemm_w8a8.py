@@ -24,7 +24,8 @@ operands of an 8-bit product are contiguous along the summed dimension. Codes
 are stored with rows a multiple of 16 bytes apart, which the kernels' bulk
 loads need; ``quantize_rows`` returns such tensors (a view of its first ``K``
 columns when ``K`` is not a multiple of 16), and a product copies operands laid
-out otherwise. Codes carry no gradient.
+out otherwise. Everything here is for inference: neither codes nor products have
+autograd history, whatever the inputs have; an ``out`` counts as modified in place.
 """
 
 from __future__ import annotations
@@ -88,6 +89,13 @@ def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+def written(t: torch.Tensor | None) -> None:
+    """Tell autograd that a caller's tensor has new contents: a backward pass that
+    saved the old ones then fails (inference tensors are not counted)."""
+    if t is not None and not t.is_inference():
+        torch.autograd.graph.increment_version(t)
 
 
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.int8
@@ -233,6 +241,7 @@ def w8a8_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scale
             a.data_ptr(), _lib.dtype_code(a.dtype), lda, sa.data_ptr(), w.data_ptr(), ldw,
             sw.data_ptr(), _lib.ptr(b), M, N, K, y.data_ptr(), _lib.dtype_code(out_dtype), N,
             _lib.stream_of(a)), "w8a8_gemm")
+    written(out)
     return y
 
 
@@ -281,4 +290,5 @@ def w8a8_gated_gemm(a8: torch.Tensor, a_scale: torch.Tensor, w_gate: torch.Tenso
             a.data_ptr(), _lib.dtype_code(a.dtype), lda, sa.data_ptr(), g.data_ptr(), ldg,
             sg.data_ptr(), u.data_ptr(), ldu, su.data_ptr(), ACTIVATIONS[activation], M, N, K,
             y.data_ptr(), _lib.dtype_code(out_dtype), N, _lib.stream_of(a)), "w8a8_gated_gemm")
+    written(out)
     return y

@@ -21,7 +21,8 @@ keeps each layer's weight as packed int4 codes plus group scales and runs
 one scale per output channel and quantizes its input per token on every call;
 ``W8A8GatedMLP`` runs a gated feed-forward block on such weights: norm with the
 residual's addition, both input projections with the activation and product in
-one kernel, and the output projection. Quantized weights take no gradient.
+one kernel, and the output projection. Quantized weights take no gradient, and
+W8A8 layers pass none on to their inputs.
 
 ``quantize_linear_layers(model)`` swaps every (or every selected) ``nn.Linear``
 of a module tree for a ``W4A16Linear`` (or, with ``scheme="w8a8"``, a
@@ -146,7 +147,10 @@ class W4A16Linear(nn.Module):
 
 class W8A8Linear(nn.Module):
     """``y = x @ W^T + b`` with W in 8-bit codes, one scale per output channel,
-    and x quantized to the same 8-bit type per row (token) on every call."""
+    and x quantized to the same 8-bit type per row (token) on every call.
+
+    For inference: the output has no autograd history even where ``x`` has one, so
+    nothing before the layer gets a gradient through it."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True,
                  dtype: torch.dtype = torch.int8,
@@ -227,7 +231,8 @@ class W8A8GatedMLP(nn.Module):
     when the block holds a norm weight.
 
     Four launches a call: the norm (or the quantizer) that writes 8-bit rows, the
-    gated product, the quantizer of its result, and the output product.
+    gated product, the quantizer of its result, and the output product. For
+    inference: neither the output nor ``h`` has autograd history.
     """
 
     def __init__(self, gate: W8A8Linear, up: W8A8Linear, down: W8A8Linear,

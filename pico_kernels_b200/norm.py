@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .gemm_w8a8 import (_FLOATS, as_rows, check_codes_dtype, check_rows, empty_rows, overlaps,
-                        row_pitch)
+                        row_pitch, written)
 
 __all__ = ["rms_norm_quant"]
 
@@ -32,6 +32,9 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     when given (contiguous, like ``x``; ``x`` or ``residual`` itself updates
     the stream in place). A row that holds a NaN or an infinity gets scale NaN
     and codes 0.
+
+    For inference: no gradient passes, ``h`` comes without autograd history even
+    where ``x`` or ``residual`` has one. ``residual_out`` counts as modified in place.
     """
     tf = _lib.torch_fast()
     if tf is not None:
@@ -87,4 +90,5 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
                 weight.data_ptr(), _lib.dtype_code(weight.dtype), eps, _lib.ptr(h), K,
                 q.data_ptr(), _lib.dtype_code(dtype), row_pitch(K), scale.data_ptr(),
                 _lib.stream_of(x)), "rms_norm_quant")
+        written(residual_out)
     return (q, scale) if h is None else (q, scale, h)

@@ -526,3 +526,35 @@ def test_out_beside_and_over_operands():
                 pk.w8a8_gated_gemm(va, vsa, vw, vsw, vu, vsu, out_dtype=torch.bfloat16, out=out(0))
         finally:
             _lib._tfast = saved
+
+
+def test_outputs_written_in_place_are_seen_by_autograd():
+    """A tensor that an earlier operation saved and a call then overwrites makes that
+    operation's backward an error, on both paths; inference tensors are written
+    as any other."""
+    a, sa, (w, sw, u, su), _ = _operands(8, 16, 32, torch.int8, weights=2)
+    x, g = torch.randn(8, 64, device="cuda").bfloat16(), torch.ones(64, device="cuda")
+    calls = [((8, 64), lambda o: pk.rms_norm_quant(x, g, residual=o, residual_out=o)),
+             ((8, 64), lambda o: pk.rms_norm_quant(x, g, residual=x, residual_out=o)),
+             ((8, 16), lambda o: pk.w8a8_gemm(a, sa, w, sw, out_dtype=torch.bfloat16, out=o)),
+             ((8, 16), lambda o: pk.w8a8_gated_gemm(a, sa, w, sw, u, su, out_dtype=torch.bfloat16,
+                                                    out=o))]
+    saved = _lib._tfast
+    for fast in (saved, False):
+        _lib._tfast = fast
+        try:
+            for shape, call in calls:
+                p = torch.randn(shape, device="cuda").bfloat16().requires_grad_()
+                h = p * 1
+                loss = h.square().sum()
+                version = h._version
+                call(h)
+                assert h._version == version + 1
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    loss.backward()
+                with torch.inference_mode():
+                    buf = torch.ones(shape, device="cuda", dtype=torch.bfloat16)
+                    call(buf)
+                call(buf)
+        finally:
+            _lib._tfast = saved
