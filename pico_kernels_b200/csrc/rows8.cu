@@ -9,7 +9,7 @@
 //
 // All three are bound by HBM: a row is read once, kept while its sum and its
 // largest magnitude are reduced, and written once (4096 x 28672 bf16 to e4m3
-// 57 us = 6.1 TB/s; the norm of 4096 x 8192 with a residual 40 us = 5.9 TB/s,
+// 54 us = 6.5 TB/s; the norm of 4096 x 8192 with a residual 40 us = 5.9 TB/s,
 // without one 23.6 us = 4.3 TB/s, where about 16 instructions a value and the
 // reduction's round trip between a row's passes take longer than its bytes).
 // The norm needs one reduction, not two (the sum for r, then the maximum of y): r multiplies
@@ -315,8 +315,8 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
 // itself): with the factor as one fp32 number a quotient that is a half step of
 // the codes came out beside it, and values of 16 bits hit half steps often. It
 // costs a packed multiplication per two values, and int8 a packed addition (codes
-// 4096 x 28672 55.2 -> 57.3 us, 4096 x 11008 22.1 -> 23.8; the norm of 4096 x 8192
-// 22.5 -> 23.6, with a residual nothing).
+// 4096 x 11008 22.1 -> 23.8 us; the norm of 4096 x 8192 22.5 -> 23.6, with a residual
+// nothing).
 __device__ __forceinline__ uint64_t quotients2(float a, float b, Factor f) {
   const uint64_t u = pack2(a, b);
   uint64_t r;
@@ -341,6 +341,18 @@ __device__ __forceinline__ uint32_t int8_codes4(const float* u, Factor f) {
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+
+// Largest |value| of both halves of two words of a 16-bit type, NaN if one is; the
+// signs of the result mean nothing.
+template <typename T>
+__device__ __forceinline__ uint32_t max2_abs(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -731,10 +743,26 @@ __global__ void __maxnreg__(thread_regs(sm_threads(kMode, kWhole, kHeld)))
       }
       if constexpr (kEarly) fetch(row + p.stages * step, stage);
     } else {
+      // (whole chunks.) The quantizer takes the maximum of 16-bit values two at a time
+      // as they lie: one instruction where unpacking them first took three (4096 x
+      // 28672 57.1 -> 54.3 us; rows that are held have to be unpacked anyway).
+      constexpr bool kPacked = !kNorm && kSize == 2;
+      uint32_t big2 = 0;
 #pragma unroll 2
       for (int c0 = t * 8; c0 < cols; c0 += lanes * 8) {
-        values(chunk(c0, std::true_type{}), c0, held[0], sum);
-        big = largest(big, held[0]);
+        const Eight<T> e = chunk(c0, std::true_type{});
+        if constexpr (kPacked) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big2 = max2_abs<T>(big2, e.w[i]);
+        } else {
+          values(e, c0, held[0], sum);
+          big = largest(big, held[0]);
+        }
+      }
+      if constexpr (kPacked) {
+        float v[8];
+        Eight<T>{big2, 0u, 0u, 0u}.values(v);
+        big = max3_abs(0.0f, v[0], v[1]);
       }
     }
     reduce_row<kNorm>(lanes, sum, big, most, s_sum[parity], s_max[parity]);

@@ -458,3 +458,20 @@ def test_norm_of_products_past_fp32(cols, residual):
         else:
             q, s = pk.rms_norm_quant(h, v, eps)
         _check_codes(q, s, _norm64(h, v, eps), 8, tol)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_a_nan_or_infinity_at_either_place_of_a_packed_pair(dt, bad):
+    x = _x(6, 20000, dt)
+    clean = pk.quantize_rows(x)
+    for at in (0, 1, 7, 4098, 19998, 19999):
+        y = x.clone()
+        y[3, at] = bad
+        y[1, at] = -y[1].abs().max() * 2  # the largest, with a sign
+        q, s = pk.quantize_rows(y)
+        assert torch.isnan(s[3]) and q[3].abs().max() == 0
+        most = -y[1, at].item() / 127
+        assert abs(s[1].item() - most) <= U * most and q[1, at] == -127
+        for i in (0, 2, 4, 5):
+            assert torch.equal(q[i], clean[0][i]) and s[i] == clean[1][i]
