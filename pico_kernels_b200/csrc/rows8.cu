@@ -268,7 +268,8 @@ __device__ __forceinline__ void store_row8(T* row, int c0, int cols, const Eight
 // lane the chunk after its neighbour's (`first`, `last`: a lane without a
 // neighbour below or above it in the row): the 16-byte blocks that hold the end
 // of its own chunk and the start of the next lane's, and single values only
-// where no block is. Norm with a residual, 5000 x 5001 bf16: 60 us, by single
+// where no block is. Norm with a residual, 5000 x 5001 bf16: 63 us (60 when the two
+// were compared), by single
 // values 86; in fp32 single values are faster (3000 x 1001: 21.7 us, so 28.2).
 template <typename T>
 __device__ __forceinline__ void store_shifted8(T* row, int c0, int cols, const Eight<T>& e,
