@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   // ---------------- split-K reduction and output ----------------
+  tc_fence_before();
   fail = __syncthreads_or(fail) != 0;
   bool stored = false;  // this thread wrote output (sharded exchange: fence before arriving)
   if (use_cluster) {
@@ -295,7 +296,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int m = 0; m < NA; ++m)
         if (m < M) red[m * kBN + nl] = acc[m];
     }
-    cluster_sync();
+    // The sums are in registers and shared memory: the columns go back before the wait
+    // for the cluster, so that no CTA of another stream's cluster waits for them
+    // while its peer holds what this one's peer needs.
+    __syncwarp();
+    cluster_arrive();
+    if (!fail && warp == kMmaWarp) {
+      tc_fence_after();
+      tmem_dealloc(tmem, C::kTmemCols);
+    }
+    __syncwarp();
+    cluster_wait();
     if (!fail && warp < kEpiWarps) {
       const int total = M * kBN;
       const int lo = (ks * total) / split, hi = ((ks + 1) * total) / split;
@@ -368,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == kMmaWarp && (fail || !use_cluster)) tmem_dealloc(tmem, C::kTmemCols);
   if (peers.world > 1) {
     if (use_cluster) {
       // every CTA of the cluster has stored its share of the columns: one
